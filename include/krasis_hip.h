@@ -591,6 +591,34 @@ size_t kr_serve_device_bytes(const kr_serve* s);
 int kr_serve_set_profiling(kr_serve* s, int enable);
 int kr_serve_get_profile(kr_serve* s, double* ms_by_family, int n);
 
+/* ---- operators over a caller's paged key / value cache (krasis_amd.kv_cache: PagedKVCache, KVBatch) ----
+ * Pages of one layer: [n_pages][page_tokens][kv_heads][dim] in a format; the microscaled ones hold codes (E4M3, or E2M1 with the even channel in the low half of a byte) and one E8M0
+ * scale byte for every 32 channels, [n_pages][page_tokens][kv_heads][dim / 32].  dim: a multiple of 32 up to 256, for attention 64, 96, 128, 192 or 256.
+ * A plan is what the calls of one step share: kr_kv_plan fills it on the host (`ints` integers; with plan = NULL it only tells how many are needed), the caller copies it to the device
+ * and passes both.  lens: stored tokens of every sequence, the counts[b] new ones at the end among them; tables: the sequences' page ids one after the other, table_lens[b] of each.
+ * Calls read the host plan before they return and only enqueue work on `stream` (of the current device; NULL or (void*)1: the default stream); they synchronise nothing and may be
+ * captured.  Pointers to pages, rows, queries, output and workspace are device pointers, aligned to 16 bytes. */
+#define KR_KV_BF16 0
+#define KR_KV_F16 1
+#define KR_KV_E4M3 2   /* round to nearest even, magnitudes over 464 become NaN */
+#define KR_KV_MX8 3    /* E4M3 times 2^s, s the smallest with max|x| <= 448 2^s, s >= -100; blocks with a NaN or an infinity read back as NaN */
+#define KR_KV_MX4 4    /* E2M1 times 2^s, 6 2^s likewise */
+typedef struct kr_kv_pages { void *k, *v, *k_scale, *v_scale; int format, page_tokens, n_pages, kv_heads, dim; } kr_kv_pages;
+int kr_kv_plan(int n_pages, int page_tokens, int batch, const int* lens, const int* counts, const int* tables, const int* table_lens, int* plan, size_t ints, size_t* need);
+/* the new rows [rows][kv_heads][dim] of bf16 / f16 (dtype KR_KV_BF16 / KR_KV_F16) into the pages, and back.  strides: {k token, k head, v token, v head} in elements, multiples of 8 */
+int kr_kv_write(const kr_kv_pages* pages, const int* plan, const int* dev_plan, const void* k, const void* v, const int64_t* strides, int dtype, void* stream);
+int kr_kv_read(const kr_kv_pages* pages, const int* plan, const int* dev_plan, void* k, void* v, const int64_t* strides, int dtype, void* stream);
+/* Attention of the new rows over the pages: out [rows][heads][dim] = softmax(scale q k) v over the keys a row sees, itself among them.  Row i of a sequence stands at position p_i = its
+ * place in the sequence; it sees key j at p_j <= p_i when window = 0, p_i - p_j < window or p_j < keep_first.  parents != NULL ([rows] on the device): the new tokens are drafts, each the
+ * child of an earlier draft of its sequence (its number there) or, -1, of the last token before them; a draft stands at its depth after that token and sees itself, its ancestors and
+ * what is before them; at most 64 a sequence.  q_token_stride, q_head_stride in elements, multiples of 8. */
+int kr_kv_attend_workspace(const kr_kv_pages* pages, const int* plan, int heads, int window, int keep_first, int tree, size_t* bytes);
+int kr_kv_attend(const kr_kv_pages* pages, const int* plan, const int* dev_plan, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int dtype, int heads, float scale,
+                 int window, int keep_first, const int* parents, void* workspace, size_t workspace_bytes, void* stream);
+/* rows moved from slot to slot (page * page_tokens + offset) in `layers` layers that lie one after the other from `pages` on: sequence b moves src[i] to dst[i] for i from start[b] to
+ * start[b + 1], in that order (start [n_seq + 1]; device pointers) */
+int kr_kv_move(const kr_kv_pages* pages, int layers, int n_seq, const int* dev_start, const int* dev_src, const int* dev_dst, void* stream);
+
 /* ---- measurement hooks (bench.py): HIP events around each kernel launch on the launch stream ----
  * kinds: 0 gate and up products, 1 down projections, 2 weighted sums (none where a call of one row forms its sum in the down projection).  Enabling profiling serialises calls. */
 int kr_set_profiling(kr_engine* e, int enable);

@@ -31,6 +31,7 @@ SYMBOLS = [
     "kr_serve_slot_len", "kr_serve_free_pages", "kr_serve_step", "kr_serve_sample", "kr_serve_set_capture", "kr_serve_read_capture", "kr_serve_device_bytes",
     "kr_serve_set_profiling", "kr_serve_get_profile", "kr_serve_set_use_graph", "kr_serve_graph_replays", "kr_serve_abi",
     "kr_serve_rows_alloc", "kr_serve_rows_free",
+    "kr_kv_plan", "kr_kv_write", "kr_kv_read", "kr_kv_attend_workspace", "kr_kv_attend", "kr_kv_move",
 ]
 TOKEN_CB = C.CFUNCTYPE(C.c_int, C.c_int, C.c_int, C.c_void_p)      # kr_token_cb(token, finish_reason, user) -> continue?
 
@@ -70,6 +71,11 @@ class ServeLayerC(C.Structure):
                 ("mix_scale", C.c_float), ("side_scale", C.c_float),
                 ("expert_in_weight", C.c_int), ("rg_width", C.c_int), ("rg_blocks", C.c_int), ("rg_conv", C.c_int), ("rg_rate", C.c_float),
                 ("keep_first", C.c_int), ("ff_bias", C.c_int), ("lt_heads", C.c_int), ("lt_dim", C.c_int), ("lt_vdim", C.c_int)]
+
+
+class KvPagesC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("format", C.c_int), ("page_tokens", C.c_int),
+                ("n_pages", C.c_int), ("kv_heads", C.c_int), ("dim", C.c_int)]
 
 
 SERVE_ABI = 6      # layout version of the two structures above (KR_SERVE_ABI in include/krasis_hip.h)
@@ -268,6 +274,12 @@ def load_library() -> C.CDLL:
     lib.kr_decode_moe_route.argtypes = [vp, ci, vp, vp, vp, ci, ci, ci]
     lib.kr_decode_num_route_weights.argtypes = [vp]
     lib.kr_decode_weight_bytes.argtypes = [vp, ci]; lib.kr_decode_weight_bytes.restype = C.c_size_t
+    i64, sz = C.c_int64, C.c_size_t
+    lib.kr_kv_plan.argtypes = [ci, ci, ci, vp, vp, vp, vp, vp, sz, C.POINTER(sz)]
+    lib.kr_kv_write.argtypes = lib.kr_kv_read.argtypes = [vp, vp, vp, vp, vp, vp, ci, vp]
+    lib.kr_kv_attend_workspace.argtypes = [vp, vp, ci, ci, ci, ci, C.POINTER(sz)]
+    lib.kr_kv_attend.argtypes = [vp, vp, vp, vp, i64, i64, vp, ci, ci, cf, ci, ci, vp, vp, sz, vp]
+    lib.kr_kv_move.argtypes = [vp, ci, ci, vp, vp, vp, vp]
     if hasattr(lib, "kr_serve_abi"):
         _bind_serve(lib)
     _lib = lib

@@ -1,0 +1,62 @@
+// kr_kv.h -- operators over a caller's paged key / value cache (krasis_amd.kv_cache.PagedKVCache): what the entry points in kr_kv.cpp hand to the kernels in kr_kv_store.hip
+// (rows quantised into the pages, read back, moved), kr_kv_step.hip and kr_kv_tile.hip (attention over the pages).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/krasis_hip.h"
+
+// one layer's pages: keys / values [slots][kv_heads][dim] in the page format, scales [slots][kv_heads][dim / 32] for the microscaled ones; slot = page * page_tokens + offset
+struct KvPages {
+    uint8_t *k, *v, *ks, *vs;
+    int row_bytes, srow_bytes;         // bytes of a slot: all heads' codes / scales
+    int head_bytes, shead_bytes;       // bytes of one head of a slot
+    int page_tokens;
+    uint32_t page_magic;               // floor(2^32 / page_tokens), at most 2^32 - 1: kv_page() below
+};
+// the sequences of a step, on the device
+struct KvSeqs {
+    const int *row0, *lens, *page0, *pages, *slots;      // [batch + 1] first new row, [batch] stored tokens with the new ones, [batch] first entry in pages, page ids, [rows] slots of the new rows
+    int batch, rows;
+};
+
+struct KvRowsArgs { KvPages p; const int* slots; void *k, *v; long k_tok, k_head, v_tok, v_head; int rows, kv_heads, dim, format, half; };      // strides in elements; half: rows are f16
+struct KvMoveArgs { uint8_t* base[4]; long layer_bytes[4]; int row_bytes[4]; const int *start, *src, *dst; int n_seq, layers; };
+
+struct KvAttnArgs {
+    KvPages p;
+    KvSeqs s;
+    const uint16_t* q; uint16_t* out;
+    long q_tok, q_head;                // strides in elements; out is [rows][heads][dim]
+    const int* parents;                // drafted trees: parent draft of every new row, or NULL
+    int heads, kv_heads, G;            // G = heads / kv_heads
+    int window, first;
+    float scale_log2;                  // scale * log2(e): scores are kept in units of log 2
+    int min_rows, max_rows;            // the sequences of this launch: those whose new rows times G lie in between
+    int tps;                           // key tiles a workgroup takes at most
+    int items;
+    float* ws;                         // partial results of sequences that are split: [item][KV_BM rows][dim] sums, then [item][rows][2] maximum and denominator
+};
+
+int kr_launch_kv_write(const KvRowsArgs& a, hipStream_t st);
+int kr_launch_kv_read(const KvRowsArgs& a, hipStream_t st);
+int kr_launch_kv_move(const KvMoveArgs& a, hipStream_t st);
+// fmt: 0 16-bit pages, 1 eight bits, 2 four bits; half: q and out are f16
+int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st);
+int kr_launch_kv_tile(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st);
+int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int half, hipStream_t st);
+
+constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step.hip
+constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile.hip
+constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
+
+// ---- the division of a launch into items, the same on the host (how many) and on the device (which one)
+// key tiles that any row tile of a sequence can need; BM rows and KT keys a tile
+__host__ __device__ inline int kv_tiles_ub(int len, int cnt, int G, int window, int first, bool tree, int bm, int kt) {
+    const int all = (len + kt - 1) / kt;
+    if (window <= 0) return all;
+    const long span = (long)window + (tree ? cnt : (bm - 1) / G + 1);      // tokens from the first row's window to the last row
+    const int some = (int)((span < len ? span : len) / kt) + 2 + (first + kt - 1) / kt;
+    return some < all ? some : all;
+}
+__host__ __device__ inline int kv_row_tiles(int cnt, int G, int bm) { return (cnt * G + bm - 1) / bm; }

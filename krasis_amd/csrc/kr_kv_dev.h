@@ -1,0 +1,129 @@
+// kr_kv_dev.h -- device helpers of the paged-cache operators: page lookup, page formats, visibility, the search for a workgroup's sequence.
+#pragma once
+#include "kr_device.h"
+#include "kr_kv.h"
+
+typedef __bf16 kv_b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 kv_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 kv_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+typedef float kv_f16 __attribute__((ext_vector_type(16)));
+
+// j / page_tokens for 0 <= j < 2^31: the high product is short by at most one
+__device__ __forceinline__ uint32_t kv_page(const KvPages& p, uint32_t j, uint32_t& off) {
+    uint32_t n = __umulhi(j, p.page_magic);
+    off = j - n * (uint32_t)p.page_tokens;
+    if (off >= (uint32_t)p.page_tokens) { n++; off -= (uint32_t)p.page_tokens; }
+    return n;
+}
+__device__ __forceinline__ uint32_t kv_slot(const KvPages& p, const int* table, uint32_t j) {
+    uint32_t off;
+    const uint32_t n = kv_page(p, j, off);
+    return (uint32_t)table[n] * (uint32_t)p.page_tokens + off;
+}
+
+// two neighbouring codes of a dword times the scale as a packed pair of bf16.  E4M3 and E2M1 have at most four significant bits and scales are powers of two of at least 2^-100:
+// every product is exact in bf16.  A scale byte of 255 stands for a block that held a NaN or an infinity and reads back as NaN.
+template <int FMT, int SEL> __device__ __forceinline__ uint32_t kv_pair(uint32_t w, float scale) {
+    if constexpr (FMT == 1) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, SEL != 0));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+}
+__device__ __forceinline__ float kv_scale(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7FC00000u : byte << 23); }
+
+template <bool H> __device__ __forceinline__ uint32_t kv_pack(float a, float b) {      // round to nearest even
+    if constexpr (H) { kv_h2 x; x[0] = (_Float16)a; x[1] = (_Float16)b; return __builtin_bit_cast(uint32_t, x); }
+    else { kv_b2 x; x[0] = (__bf16)a; x[1] = (__bf16)b; return __builtin_bit_cast(uint32_t, x); }
+}
+__device__ __forceinline__ kv_h2 kv_halves(uint32_t w) { return __builtin_bit_cast(kv_h2, w); }      // by value: a bit cast of a vector's element takes the vector's first
+__device__ __forceinline__ float kv_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float kv_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+// what a packed pair of bf16 leaves of two floats
+__device__ __forceinline__ uint32_t kv_rest(float a, float b, uint32_t w) { return kv_pack<false>(a - kv_lo(w), b - kv_hi(w)); }
+
+// ancestors of the drafts of one sequence, lane i: bit j set when draft j is draft i or an ancestor.  Parents are doubled up: after k rounds a lane knows 2^k ancestors.
+// A parent that is no earlier draft counts as none.
+__device__ __forceinline__ uint64_t kv_ancestors(const int* parents, int n, int lane) {
+    int par = lane < n ? parents[lane] : -1;
+    if (par >= lane || par < 0) par = -1;
+    uint64_t seen = 1ull << lane;
+#pragma unroll
+    for (int r = 0; r < 6; r++) {
+        const int from = par < 0 ? lane : par;
+        const uint32_t lo = __shfl((uint32_t)seen, from), hi = __shfl((uint32_t)(seen >> 32), from);
+        const int up = __shfl(par, from);
+        if (par >= 0) { seen |= (uint64_t)hi << 32 | lo; par = up; }
+    }
+    return seen;
+}
+
+struct KvItem { int b, rt, split, kvh, nsplit, len, cnt, row0, page0, base; };      // base: the sequence's first item
+// item -> sequence, row tile, share of the keys, head.  A lane counts the items of one sequence, 64 sequences at a time; heads lie side by side (they read the same lines of scales),
+// the last row tiles first (a prompt's last rows see the most keys).  sub: parts of a row tile in a launch over row tiles alone (shares = 1).
+template <bool SHARES> __device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, int idx, int bm, int kt, int sub) {
+    const int lane = threadIdx.x & 63;
+    KvItem it;
+    int base = 0, ibase = 0;
+    for (int b0 = 0; b0 < a.s.batch; b0 += 64) {
+        const int b = b0 + lane;
+        int n = 0, full = 0, len = 0, cnt = 0, ns = 1, row0 = 0;
+        if (b < a.s.batch) {
+            row0 = a.s.row0[b]; cnt = a.s.row0[b + 1] - row0; len = a.s.lens[b];
+            const int rows = cnt * a.G;
+            if (rows >= a.min_rows && rows <= a.max_rows) {
+                ns = (kv_tiles_ub(len, cnt, a.G, a.window, a.first, a.parents != nullptr, bm, kt) + a.tps - 1) / a.tps;
+                const int rts = kv_row_tiles(cnt, a.G, bm);
+                full = rts * ns * a.kv_heads;
+                n = SHARES ? full : (ns > 1 ? rts * sub * a.kv_heads : 0);
+            }
+        }
+        int end = n, iend = full;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(end, d), y = SHARES ? 0 : __shfl_up(iend, d);
+            if (lane >= d) { end += x; iend += y; }
+        }
+        const uint64_t hit = __ballot(base + end > idx);
+        if (hit) {
+            const int w = __builtin_ctzll(hit);
+            it.b = b0 + w;
+            it.nsplit = __builtin_amdgcn_readlane(ns, w); it.len = __builtin_amdgcn_readlane(len, w); it.cnt = __builtin_amdgcn_readlane(cnt, w); it.row0 = __builtin_amdgcn_readlane(row0, w);
+            const int e = __builtin_amdgcn_readlane(end, w), nn = __builtin_amdgcn_readlane(n, w);
+            int r = idx - (base + e - nn);
+            it.base = SHARES ? base + e - nn : ibase + __builtin_amdgcn_readlane(iend, w) - __builtin_amdgcn_readlane(full, w);
+            it.kvh = r % a.kv_heads; r /= a.kv_heads;
+            const int per = SHARES ? it.nsplit : sub;
+            it.split = r % per; it.rt = kv_row_tiles(it.cnt, a.G, bm) - 1 - r / per;
+            it.page0 = a.s.page0[it.b];
+            it.page0 = __builtin_amdgcn_readfirstlane(it.page0);
+            return it;
+        }
+        base += __builtin_amdgcn_readlane(end, 63);
+        if (!SHARES) ibase += __builtin_amdgcn_readlane(iend, 63);
+    }
+    it.b = -1;
+    return it;
+}
+// the item that holds a row tile's share, for the one who joins them
+__device__ __forceinline__ int kv_item_of(const KvAttnArgs& a, const KvItem& it, int bm, int split) {
+    return it.base + ((kv_row_tiles(it.cnt, a.G, bm) - 1 - it.rt) * it.nsplit + split) * a.kv_heads + it.kvh;
+}
+
+// the keys of a row tile: tiles of kept first keys that lie apart from the window's, then one range
+struct KvRange { int lo, hi, kept, start, tiles, before, t0, t1; };      // [lo, hi) without the kept ones, tiles of kept keys, first key of the range, tiles in all
+__device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& it, int bm, int kt) {
+    KvRange r;
+    r.before = it.len - it.cnt;
+    r.t0 = it.rt * bm / a.G;
+    r.t1 = min(it.cnt, ((it.rt + 1) * bm - 1) / a.G + 1);
+    r.hi = r.before + r.t1;                  // a draft's ancestors come before it
+    r.lo = 0; r.kept = 0; r.start = 0;
+    if (a.window > 0) {
+        r.lo = max(0, r.before + (a.parents ? 0 : r.t0) - a.window + 1);
+        const int at = r.lo / kt * kt;
+        if (a.first > 0 && at < a.first) r.start = 0;
+        else { r.start = at; r.kept = (min(a.first, r.hi) + kt - 1) / kt; }
+    }
+    r.tiles = r.kept + (r.hi - r.start + kt - 1) / kt;
+    return r;
+}

@@ -1,0 +1,328 @@
+// kr_kv_step.hip -- attention over the paged cache for sequences with at most 16 rows of new tokens (one token of a group of up to 16 heads, a few tokens of smaller groups):
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the stored keys j that row i sees.
+// A row of keys serves 16 rows of queries: 4 * 16 operations a channel against one to four bytes of it, far under the matrix rate, so the launch is bound by HBM and its latency.
+// Keys and values go from the pages to registers once, converted there to bf16 (exact, kr_kv_dev.h), and meet the queries in v_mfma_f32_16x16x32:
+//   S^T[key][row] = K Q^T    first operand: 16 key rows; a lane holds a quarter of a row, so a microscaled row costs it one scale and loads of 16 bytes
+//   O^T[d][row] += V^T P^T   a lane holds 8 keys and c neighbouring columns; byte permutes make them the columns' fragments
+// A workgroup takes one sequence, one key / value head and a share of its key tiles; its four waves take tiles of 32 keys in turn, each with a running maximum and sum per row, and
+// meet in LDS.  Weights are taken as two bf16 pieces (16 bits), f16 queries over bf16-converted pages too: the matrix cores have time for it here.
+#include "kr_kv_dev.h"
+#include "kr_lds_optin.h"
+
+constexpr int KVS_WAVES = 4;
+template <int DIM> struct KvsCols { static constexpr int C = DIM == 96 ? 2 : DIM == 192 ? 4 : DIM / 16, GROUPS = DIM / (16 * C); };      // columns of V a lane holds: groups of 16 C
+inline int kvs_lds(int dim) { return (KVS_WAVES * 16 * (dim + 4) + KVS_WAVES * 32 + 32) * (int)sizeof(float); }
+
+template <int BYTES> __device__ __forceinline__ void kvs_load(const uint8_t* p, uint32_t* w) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; i++) { const u32x4 x = *reinterpret_cast<const u32x4*>(p + 16 * i); w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w; }
+    } else if constexpr (BYTES % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 8; i++) { const u32x2 x = *reinterpret_cast<const u32x2*>(p + 8 * i); w[2 * i] = x.x; w[2 * i + 1] = x.y; }
+    } else if constexpr (BYTES % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; i++) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+    } else if constexpr (BYTES == 2) w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else w[0] = *p;
+}
+// pair e of packed codes as two 16-bit numbers
+template <int FMT> __device__ __forceinline__ uint32_t kvs_two(const uint32_t* w, int e, float scale) {
+    if constexpr (FMT == 0) return w[e];
+    else if constexpr (FMT == 1) return (e & 1) ? kv_pair<1, 1>(w[e >> 1], scale) : kv_pair<1, 0>(w[e >> 1], scale);
+    else return (e & 3) == 0 ? kv_pair<2, 0>(w[e >> 2], scale) : (e & 3) == 1 ? kv_pair<2, 1>(w[e >> 2], scale) : (e & 3) == 2 ? kv_pair<2, 2>(w[e >> 2], scale) : kv_pair<2, 3>(w[e >> 2], scale);
+}
+template <bool H> __device__ __forceinline__ kv_f4 kvs_mfma(u32x4 x, u32x4 y, kv_f4 c) {
+    if constexpr (H) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv_h8, x), __builtin_bit_cast(kv_h8, y), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv_b8, x), __builtin_bit_cast(kv_b8, y), c, 0, 0, 0);
+}
+
+// HQ: q and out are f16.  Products are f16 where the pages are f16 too, else bf16.
+template <int DIM, int FMT, bool HQ>
+__global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttnArgs a) {
+    constexpr bool HM = HQ && FMT == 0;                       // f16 products
+    constexpr int QP = HQ && !HM ? 2 : 1, PP = HM ? 1 : 2;    // pieces of a query and of a weight
+    constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, U = DIM / 32, KB = DIM / 4 * BITS / 8, KW = KB / 4;
+    constexpr int C = KvsCols<DIM>::C, GROUPS = KvsCols<DIM>::GROUPS, VB = C * BITS / 8, VW = VB < 4 ? 1 : VB / 4;
+    constexpr int NB = DIM == 64 || DIM == 128 ? 1 : 2;       // blocks of 32 channels that a quarter of a row meets
+    extern __shared__ float kvs_lds_[];
+    const KvItem it = kv_item<true>(a, blockIdx.x, 16, KV_STEP_KT, 1);
+    if (it.b < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, q = lane >> 4;
+    const KvRange rg = kv_range(a, it, 16, KV_STEP_KT);
+    const int c0 = it.split * a.tps, c1 = min(rg.tiles, c0 + a.tps);
+    const int rows = it.cnt * a.G, r = min(row, rows - 1), t = r / a.G, head = it.kvh * a.G + r - t * a.G;
+    const int* table = a.s.pages + it.page0;
+    const bool scaled = FMT != 0 && a.p.ks != nullptr;
+    const uint8_t* kbase = a.p.k + (size_t)it.kvh * a.p.head_bytes + q * KB;
+    const uint8_t* vbase = a.p.v + (size_t)it.kvh * a.p.head_bytes;
+    const uint8_t* ksb = a.p.ks + (size_t)it.kvh * a.p.shead_bytes;
+    const uint8_t* vsb = a.p.vs + (size_t)it.kvh * a.p.shead_bytes;
+
+    // the row's position, and which drafts it sees
+    int pos = rg.before + t; uint64_t seen = 0; int depth = 0;
+    if (a.parents) {
+        const uint64_t all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
+        depth = __popcll(all) - 1;                            // of draft `lane`
+        seen = (uint64_t)__shfl((uint32_t)(all >> 32), t) << 32 | __shfl((uint32_t)all, t);
+        pos = rg.before + __shfl(depth, t);
+    }
+    // the query row: dims q DIM / 4 + 8 i
+    u32x4 qf[QP][U];
+    {
+        const uint16_t* qp = a.q + (size_t)(it.row0 + t) * a.q_tok + (size_t)head * a.q_head + q * (DIM / 4);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 8 * i);
+            if constexpr (QP == 1) qf[0][i] = x;
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const kv_h2 h = kv_halves(x[e]);
+                    const float u = (float)h[0], w = (float)h[1];
+                    qf[0][i][e] = kv_pack<false>(u, w); qf[1][i][e] = kv_rest(u, w, qf[0][i][e]);
+                }
+            }
+        }
+    }
+
+    uint32_t kn[2][KW], vn[8][GROUPS][VW]; uint32_t ksn[2][NB], vsn[8][GROUPS];
+    auto request = [&](int c) {
+        const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept);
+        auto key = [&](int k) { const int j = j0 + k; return j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1); };      // keys no row sees give way to one that is seen
+        const int s = (int)kv_slot(a.p, table, (uint32_t)key(lane & 31));
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const size_t sl = (uint32_t)__shfl(s, b * 16 + row);
+            kvs_load<KB>(kbase + sl * a.p.row_bytes, kn[b]);
+            if (scaled) {
+                const uint8_t* sp = ksb + sl * a.p.srow_bytes;
+                const int b0 = (q * U) >> 2;
+#pragma unroll
+                for (int i = 0; i < NB; i++) ksn[b][i] = sp[min(b0 + i, DIM / 32 - 1)];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const size_t sl = (uint32_t)__shfl(s, (i >> 2) * 16 + 4 * q + (i & 3));
+            const uint8_t* vp = vbase + sl * a.p.row_bytes + row * VB;
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) kvs_load<VB>(vp + g * 16 * VB, vn[i][g]);
+            if (scaled) {
+                const uint8_t* sp = vsb + sl * a.p.srow_bytes;
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) vsn[i][g] = sp[(g * 16 * C + row * C) / 32];
+            }
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    kv_f4 acc[DIM / 16];
+#pragma unroll
+    for (int j = 0; j < DIM / 16; j++) acc[j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (c0 + wave < c1) request(c0 + wave);
+    for (int c = c0 + wave; c < c1; c += KVS_WAVES) {
+        const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept), end = c < rg.kept ? min(a.first, rg.hi) : rg.hi;
+        kv_f4 st[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            st[b] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            float sc[NB];
+#pragma unroll
+            for (int i = 0; i < NB; i++) sc[i] = scaled ? kv_scale(ksn[b][i]) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                float s = sc[0];
+                if constexpr (NB == 2) { if (DIM == 256 ? i >= 4 : ((q * U + i) >> 2) != (q * U) >> 2) s = sc[1]; }
+                u32x4 kf;
+#pragma unroll
+                for (int e = 0; e < 4; e++) kf[e] = kvs_two<FMT>(&kn[b][i * KW / U], e, s);
+#pragma unroll
+                for (int p = QP - 1; p >= 0; p--) st[b] = kvs_mfma<HM>(kf, qf[p][i], st[b]);
+            }
+        }
+        uint32_t vv[8][GROUPS][C / 2];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                const float s = scaled ? kv_scale(vsn[i][g]) : 1.0f;
+#pragma unroll
+                for (int e = 0; e < C / 2; e++) vv[i][g][e] = kvs_two<FMT>(vn[i][g], e, s);
+            }
+        if (c + KVS_WAVES < c1) request(c + KVS_WAVES);
+        float cm = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = j0 + b * 16 + 4 * q + i;
+                int at = key; bool ok = key < end;
+                if (a.parents) {
+                    const int n = key - rg.before, d = __shfl(depth, n & 63);
+                    if (n >= 0) { at = rg.before + d; ok = ok && (seen >> (n & 63) & 1); }
+                } else ok = ok && key <= pos;
+                if (a.window > 0) ok = ok && (pos - at < a.window || at < a.first);
+                st[b][i] = ok ? st[b][i] * a.scale_log2 : -INFINITY;
+                cm = fmaxf(cm, st[b][i]);
+            }
+        cm = fmaxf(cm, __shfl_xor(cm, 16)); cm = fmaxf(cm, __shfl_xor(cm, 32));
+        const float mn = fmaxf(m, cm), base = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - base);
+        m = mn; l *= alpha;
+        u32x4 pf[PP];
+        uint32_t vis[4];                                      // ones where the row sees the key, as a fragment
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float s0 = st[e >> 1][2 * (e & 1)], s1 = st[e >> 1][2 * (e & 1) + 1];
+            const float p0 = __builtin_amdgcn_exp2f(s0 - base), p1 = __builtin_amdgcn_exp2f(s1 - base);
+            l += p0 + p1;
+            pf[0][e] = kv_pack<HM>(p0, p1);
+            if constexpr (PP == 2) pf[1][e] = kv_rest(p0, p1, pf[0][e]);
+            vis[e] = (s0 == -INFINITY ? 0u : (HM ? 0x3C00u : 0x3F80u)) | (s1 == -INFINITY ? 0u : (HM ? 0x3C000000u : 0x3F800000u));
+        }
+        constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, ONE = HM ? 0x3C00u : 0x3F80u;
+        // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys: nothing to do, but for an
+        // infinity (16-bit pages hold them) and a weight whose second piece is 0 or negative.
+        bool odd = false;
+        if (it.cnt > 1 || (FMT == 0 && PP == 2)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+                    for (int e = 0; e < C / 2; e++) odd = odd || (vv[i][g][e] & EXP) == EXP || (vv[i][g][e] >> 16 & EXP) == EXP;
+            odd = __any(odd);
+        }
+#pragma unroll
+        for (int j = 0; j < DIM / 16; j++) {
+            u32x4 vf;
+#pragma unroll
+            for (int e = 0; e < 4; e++) vf[e] = __builtin_amdgcn_perm(vv[2 * e + 1][j / C][j % C / 2], vv[2 * e][j / C][j % C / 2], (j & 1) ? 0x07060302u : 0x05040100u);
+            acc[j] *= alpha;
+            if (odd) {                                        // such values apart: how many of them a row sees, by kind
+                u32x4 kind[3];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t keep = 0; kind[0][e] = kind[1][e] = kind[2][e] = 0;
+#pragma unroll
+                    for (int h = 0; h < 32; h += 16) {
+                        const uint32_t x = vf[e] >> h & 0xFFFFu;
+                        if ((x & EXP) != EXP) keep |= x << h;
+                        else if (x & (HM ? 0x3FFu : 0x7Fu)) kind[2][e] |= ONE << h;
+                        else if (x & 0x8000u) kind[1][e] |= ONE << h;
+                        else kind[0][e] |= ONE << h;
+                    }
+                    vf[e] = keep;
+                }
+                const u32x4 see = {vis[0], vis[1], vis[2], vis[3]};
+                const kv_f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                const kv_f4 up = kvs_mfma<HM>(kind[0], see, zero), down = kvs_mfma<HM>(kind[1], see, zero), nan = kvs_mfma<HM>(kind[2], see, zero);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (up[i] > 0.0f) acc[j][i] += INFINITY;
+                    if (down[i] > 0.0f) acc[j][i] -= INFINITY;
+                    if (nan[i] > 0.0f) acc[j][i] = NAN;
+                }
+            }
+#pragma unroll
+            for (int p = PP - 1; p >= 0; p--) acc[j] = kvs_mfma<HM>(vf, pf[p], acc[j]);
+        }
+    }
+    // ---- the waves' states meet: [waves][16][DIM + 4] sums | [waves][16] maxima | [waves][16] denominators | [16] maximum | [16] denominator
+    constexpr int VS = DIM + 4;
+    float* ml = kvs_lds_ + KVS_WAVES * 16 * VS; float* dl = ml + KVS_WAVES * 16; float* mt = dl + KVS_WAVES * 16; float* dt = mt + 16;
+    l += __shfl_xor(l, 16); l += __shfl_xor(l, 32);
+    if (q == 0) { ml[wave * 16 + row] = m; dl[wave * 16 + row] = l; }
+    __syncthreads();
+    float top = -INFINITY, den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < KVS_WAVES; w++) top = fmaxf(top, ml[w * 16 + row]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < KVS_WAVES; w++) den += dl[w * 16 + row] * __builtin_amdgcn_exp2f(ml[w * 16 + row] - base);
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    float* mine = kvs_lds_ + (wave * 16 + row) * VS;
+#pragma unroll
+    for (int j = 0; j < DIM / 16; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mine[j / C * 16 * C + (4 * q + i) * C + j % C] = m == -INFINITY ? 0.0f : acc[j][i] * f;
+    if (tid < 16) { mt[tid] = top; dt[tid] = den; }
+    __syncthreads();
+    const bool whole = it.nsplit == 1;
+    float* wo = a.ws + (size_t)blockIdx.x * 16 * DIM;
+    for (int i = tid; i < rows * (DIM / 4); i += 64 * KVS_WAVES) {
+        const int rr = i / (DIM / 4), d = (i - rr * (DIM / 4)) * 4;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < KVS_WAVES; w++) {
+            const float4 x = *reinterpret_cast<const float4*>(kvs_lds_ + (w * 16 + rr) * VS + d);
+            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+        if (whole) {
+            const float inv = dt[rr] == 0.0f ? 0.0f : 1.0f / dt[rr];
+            const int tt = rr / a.G, hh = it.kvh * a.G + rr - tt * a.G;
+            u32x2 o = {kv_pack<HQ>(s.x * inv, s.y * inv), kv_pack<HQ>(s.z * inv, s.w * inv)};
+            *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + tt) * a.heads + hh) * DIM + d) = o;
+        } else *reinterpret_cast<float4*>(wo + rr * DIM + d) = s;
+    }
+    if (!whole && tid < 16) {
+        float* st = a.ws + (size_t)a.items * 16 * DIM + ((size_t)blockIdx.x * 16 + tid) * 2;
+        st[0] = mt[tid]; st[1] = dt[tid];
+    }
+}
+
+template <int DIM, int FMT> static int kvs_launch(const KvAttnArgs& a, int half, hipStream_t st) {
+    const size_t lds = kvs_lds(DIM);
+    const void* fn = half ? (const void*)kr_kv_step_kernel<DIM, FMT, true> : (const void*)kr_kv_step_kernel<DIM, FMT, false>;
+    if (lds > 65536 && kr_lds_optin(fn, lds)) return 1;
+    if (half) hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, true>), dim3(a.items), dim3(64 * KVS_WAVES), lds, st, a);
+    else hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, false>), dim3(a.items), dim3(64 * KVS_WAVES), lds, st, a);
+    return 0;
+}
+template <int FMT> static int kvs_dim(const KvAttnArgs& a, int dim, int half, hipStream_t st) {
+    switch (dim) {
+        case 64: return kvs_launch<64, FMT>(a, half, st);
+        case 96: return kvs_launch<96, FMT>(a, half, st);
+        case 128: return kvs_launch<128, FMT>(a, half, st);
+        case 192: return kvs_launch<192, FMT>(a, half, st);
+        case 256: return kvs_launch<256, FMT>(a, half, st);
+    }
+    return 1;
+}
+int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st) {
+    return fmt == 0 ? kvs_dim<0>(a, dim, half, st) : fmt == 1 ? kvs_dim<1>(a, dim, half, st) : kvs_dim<2>(a, dim, half, st);
+}
+
+// Shares of split sequences joined: unit = 16 rows of a row tile of bm rows and one head; a thread holds four columns of a row.
+template <bool H> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
+    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, bm / 16);
+    if (it.b < 0) return;
+    const int rows = it.cnt * a.G, quads = dim / 4;
+    const float* stats = a.ws + (size_t)a.items * bm * dim;
+    for (int i = threadIdx.x; i < 16 * quads; i += 256) {
+        const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
+        if (rr >= rows) continue;
+        float top = -INFINITY;
+        for (int s = 0; s < it.nsplit; s++) top = fmaxf(top, stats[((size_t)kv_item_of(a, it, bm, s) * bm + r) * 2]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < it.nsplit; s++) {
+            const size_t at = (size_t)kv_item_of(a, it, bm, s) * bm + r;
+            const float ms = stats[at * 2], f = __builtin_amdgcn_exp2f(ms - base), ls = stats[at * 2 + 1];
+            const float4 x = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
+            if (ms == -INFINITY && ls == 0.0f) continue;      // a share without keys of this row
+            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+            den += ls * f;
+        }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
+        u32x2 w = {kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
+        *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = w;
+    }
+}
+int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int half, hipStream_t st) {
+    if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+    else hipLaunchKernelGGL((kr_kv_join_kernel<false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+    return 0;
+}
