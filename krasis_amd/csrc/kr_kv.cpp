@@ -19,6 +19,7 @@ struct Plan {
     }
 };
 int bits_of(int format) { return format == KR_KV_BF16 || format == KR_KV_F16 ? 16 : format == KR_KV_E4M3 || format == KR_KV_MX8 ? 8 : 4; }
+int fmt_of(int format) { return bits_of(format) == 16 ? 0 : bits_of(format) == 8 ? 1 : 2; }
 bool scaled(int format) { return format == KR_KV_MX8 || format == KR_KV_MX4; }
 bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
@@ -70,32 +71,53 @@ int rows_call(const char* what, const kr_kv_pages* p, const int* plan, const int
 }
 
 // one launch's share of a call: the sequences whose rows (new tokens x heads of a group) lie in a range
-struct Part { int min_rows, max_rows, bm, kt, tps; int64_t items, units; bool split; };
-// Key tiles are shared out so that `target` workgroups, what the chip holds at once, have some; a share is at least `least` tiles, below which joining costs more than it saves.
-void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int target, int least, Part& p) {
-    int64_t total = 0;
+struct Part { int min_rows, max_rows, bm, kt, tps; int64_t items, units; int shares; bool split, few, one; };
+// How many key tiles a workgroup takes: `hold` workgroups are on the chip at once, so the launch lasts rounds * (tiles a workgroup + what it takes to begin and to end, `extra` tiles),
+// and the cheapest number of rounds up to four is taken (more items than that without any sharing out: they fill the chip evenly by themselves).
+void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int hold, int least, int extra, Part& p) {
+    struct Seq { int tiles; int64_t row_tiles; };
+    std::vector<Seq> seqs;
+    int64_t total = 0, whole = 0; int longest = 0;
     for (int b = 0; b < h.batch; b++) {
         const int cnt = h.row0[b + 1] - h.row0[b]; const int64_t rows = (int64_t)cnt * G;
         if (rows < p.min_rows || rows > p.max_rows) continue;
-        total += (int64_t)kv_row_tiles(cnt, G, p.bm) * kv_heads * kv_tiles_ub(h.lens[b], cnt, G, window, first, tree, p.bm, p.kt);
+        const int n = kv_tiles_ub(h.lens[b], cnt, G, window, first, tree, p.bm, p.kt);
+        const int64_t rt = (int64_t)kv_row_tiles(cnt, G, p.bm) * kv_heads;
+        if (cnt > 1) p.one = false;
+        seqs.push_back({n, rt}); total += rt * n; whole += rt; longest = n > longest ? n : longest;
     }
-    const int64_t share = (total + target - 1) / target;
-    p.tps = (int)(share < least ? least : share > INT32_MAX ? INT32_MAX : share);
-    p.items = p.units = 0; p.split = false;
-    for (int b = 0; b < h.batch; b++) {
-        const int cnt = h.row0[b + 1] - h.row0[b]; const int64_t rows = (int64_t)cnt * G;
-        if (rows < p.min_rows || rows > p.max_rows) continue;
-        const int ns = (kv_tiles_ub(h.lens[b], cnt, G, window, first, tree, p.bm, p.kt) + p.tps - 1) / p.tps, rt = kv_row_tiles(cnt, G, p.bm);
-        p.items += (int64_t)rt * ns * kv_heads;
-        if (ns > 1) { p.units += (int64_t)rt * (p.bm / 16) * kv_heads; p.split = true; }
+    p.items = whole; p.units = 0; p.split = p.few = false; p.one = !tree; p.tps = longest > 0 ? longest : 1;
+    if (seqs.empty()) return;
+    auto items = [&](int tps) { int64_t n = 0; for (const Seq& s : seqs) n += s.row_tiles * ((s.tiles + tps - 1) / tps); return n; };
+    if (whole < 4ll * hold && longest > least) {
+        int64_t best = ((whole + hold - 1) / hold) * (longest + extra);
+        for (int64_t k = (whole + hold - 1) / hold; k <= 4; k++) {
+            int lo = (int)(total / (k * hold)), hi = longest;      // the smallest share whose items fit into k rounds
+            if (lo < least) lo = least;
+            if (lo < (longest + KV_MAX_SHARES - 1) / KV_MAX_SHARES) lo = (longest + KV_MAX_SHARES - 1) / KV_MAX_SHARES;
+            while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (items(mid) <= k * hold) hi = mid; else lo = mid + 1; }
+            const int64_t cost = k * (lo + extra);
+            if (lo < longest && cost < best) { best = cost; p.tps = lo; }
+        }
     }
+    int most = 1;
+    p.items = 0;
+    for (const Seq& s : seqs) {
+        const int ns = (s.tiles + p.tps - 1) / p.tps;
+        p.items += s.row_tiles * ns;
+        if (ns > 1) p.split = true;
+        most = ns > most ? ns : most;
+    }
+    p.shares = most;
+    p.few = most <= 4;
+    if (p.split) for (const Seq& s : seqs) if (s.tiles > p.tps) p.units += s.row_tiles * (p.few ? p.bm / 16 : p.bm);
 }
-void parts_of(const Plan& h, int kv_heads, int heads, int dim, int window, int first, bool tree, Part* p) {
+void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, int window, int first, bool tree, Part* p) {
     const int G = heads / kv_heads;
-    p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, false};
-    p[1] = Part{KV_STEP_BM + 1, INT32_MAX, KV_TILE_BM, KV_TILE_KT, 0, 0, 0, false};
-    divide(h, kv_heads, G, window, first, tree, dim <= 128 ? 2 * KV_CUS : KV_CUS, 4, p[0]);
-    divide(h, kv_heads, G, window, first, tree, dim <= 128 ? 2 * KV_CUS : KV_CUS, 2, p[1]);
+    p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, 1, false, false, false};
+    p[1] = Part{KV_STEP_BM + 1, INT32_MAX, KV_TILE_BM, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
+    divide(h, kv_heads, G, window, first, tree, kv_step_hold(dim, fmt) * KV_CUS, 4, 8, p[0]);
+    divide(h, kv_heads, G, window, first, tree, dim <= 128 ? 2 * KV_CUS : KV_CUS, 2, 3, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
 
@@ -175,7 +197,7 @@ extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int
     if (!bytes) return kr_fail(KR_ERR_VALUE, "kr_kv_attend_workspace: null argument");
     const Plan h(plan);
     Part part[2];
-    parts_of(h, p->kv_heads, heads, p->dim, window, clamp_first(h, window, keep_first), tree != 0, part);
+    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), window, clamp_first(h, window, keep_first), tree != 0, part);
     *bytes = part_bytes(part[0], p->dim) + part_bytes(part[1], p->dim);
     return KR_OK;
 }
@@ -197,19 +219,19 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
     a.window = window; a.first = clamp_first(h, window, keep_first);
     a.scale_log2 = scale * 1.44269504088896340736f;
     Part part[2];
-    parts_of(h, p->kv_heads, heads, p->dim, window, a.first, parents != nullptr, part);
+    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), window, a.first, parents != nullptr, part);
     const size_t b0 = part_bytes(part[0], p->dim), b1 = part_bytes(part[1], p->dim);
     if (workspace_bytes < b0 + b1 || ((b0 + b1) && (!workspace || misaligned(workspace)))) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: a workspace of %zu bytes for %zu", workspace_bytes, b0 + b1);
-    if (part[0].items > INT32_MAX || part[1].items > INT32_MAX || part[0].units > INT32_MAX || part[1].units > INT32_MAX) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: %d rows are too many for one call", h.rows);
-    const int fmt = bits_of(p->format) == 16 ? 0 : bits_of(p->format) == 8 ? 1 : 2, half = dtype == KR_KV_F16;
+    if (part[0].items > INT32_MAX || part[1].items > INT32_MAX || part[0].units > INT32_MAX || part[0].shares > KV_MAX_SHARES || part[1].shares > KV_MAX_SHARES || part[1].units > INT32_MAX) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: %d rows are too many for one call", h.rows);
+    const int fmt = fmt_of(p->format), half = dtype == KR_KV_F16;
     hipStream_t st = stream_of(stream);
     for (int i = 1; i >= 0; i--) {                            // prompts first, they take longest
         if (!part[i].items) continue;
-        a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = part[i].tps; a.items = (int)part[i].items;
+        a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = part[i].tps; a.items = (int)part[i].items; a.one = part[i].one;
         a.ws = (float*)((char*)workspace + (i ? b0 : 0));
         if (int rc = launched("kr_kv_attend", i ? kr_launch_kv_tile(a, p->dim, fmt, half, st) : kr_launch_kv_step(a, p->dim, fmt, half, st))) return rc;
         if (part[i].split)
-            if (int rc = launched("kr_kv_attend", kr_launch_kv_join(a, p->dim, part[i].bm, part[i].kt, (int)part[i].units, half, st))) return rc;
+            if (int rc = launched("kr_kv_attend", kr_launch_kv_join(a, p->dim, part[i].bm, part[i].kt, (int)part[i].units, part[i].few, half, st))) return rc;
     }
     return KR_OK;
 }

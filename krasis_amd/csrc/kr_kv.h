@@ -34,7 +34,7 @@ struct KvAttnArgs {
     float scale_log2;                  // scale * log2(e): scores are kept in units of log 2
     int min_rows, max_rows;            // the sequences of this launch: those whose new rows times G lie in between
     int tps;                           // key tiles a workgroup takes at most
-    int items;
+    int items, one;                    // one: no sequence of this launch has more than one new token, and there are no trees
     float* ws;                         // partial results of sequences that are split: [item][KV_BM rows][dim] sums, then [item][rows][2] maximum and denominator
 };
 
@@ -44,10 +44,12 @@ int kr_launch_kv_move(const KvMoveArgs& a, hipStream_t st);
 // fmt: 0 16-bit pages, 1 eight bits, 2 four bits; half: q and out are f16
 int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st);
 int kr_launch_kv_tile(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st);
-int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int half, hipStream_t st);
+int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st);
+constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 
 constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step.hip
 constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile.hip
+__host__ __device__ constexpr int kv_step_hold(int dim, int fmt) { return dim <= 128 ? 3 : dim == 256 && fmt == 0 ? 1 : 2; }      // workgroups of four waves a CU: by registers
 constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
 
 // ---- the division of a launch into items, the same on the host (how many) and on the device (which one)

@@ -66,9 +66,9 @@ template <bool SHARES> __device__ __forceinline__ KvItem kv_item(const KvAttnArg
     int base = 0, ibase = 0;
     for (int b0 = 0; b0 < a.s.batch; b0 += 64) {
         const int b = b0 + lane;
-        int n = 0, full = 0, len = 0, cnt = 0, ns = 1, row0 = 0;
+        int n = 0, full = 0, len = 0, cnt = 0, ns = 1, row0 = 0, page0 = 0;
         if (b < a.s.batch) {
-            row0 = a.s.row0[b]; cnt = a.s.row0[b + 1] - row0; len = a.s.lens[b];
+            row0 = a.s.row0[b]; cnt = a.s.row0[b + 1] - row0; len = a.s.lens[b]; page0 = a.s.page0[b];
             const int rows = cnt * a.G;
             if (rows >= a.min_rows && rows <= a.max_rows) {
                 ns = (kv_tiles_ub(len, cnt, a.G, a.window, a.first, a.parents != nullptr, bm, kt) + a.tps - 1) / a.tps;
@@ -94,8 +94,7 @@ template <bool SHARES> __device__ __forceinline__ KvItem kv_item(const KvAttnArg
             it.kvh = r % a.kv_heads; r /= a.kv_heads;
             const int per = SHARES ? it.nsplit : sub;
             it.split = r % per; it.rt = kv_row_tiles(it.cnt, a.G, bm) - 1 - r / per;
-            it.page0 = a.s.page0[it.b];
-            it.page0 = __builtin_amdgcn_readfirstlane(it.page0);
+            it.page0 = __builtin_amdgcn_readlane(page0, w);
             return it;
         }
         base += __builtin_amdgcn_readlane(end, 63);

@@ -37,9 +37,9 @@ template <bool H> __device__ __forceinline__ kv_f4 kvs_mfma(u32x4 x, u32x4 y, kv
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv_b8, x), __builtin_bit_cast(kv_b8, y), c, 0, 0, 0);
 }
 
-// HQ: q and out are f16.  Products are f16 where the pages are f16 too, else bf16.
-template <int DIM, int FMT, bool HQ>
-__global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttnArgs a) {
+// HQ: q and out are f16.  Products are f16 where the pages are f16 too, else bf16.  ONE: every sequence of the launch has one new token and no tree, so that its rows see the same keys.
+template <int DIM, int FMT, bool HQ, bool ONE>
+__global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_step_kernel(const KvAttnArgs a) {
     constexpr bool HM = HQ && FMT == 0;                       // f16 products
     constexpr int QP = HQ && !HM ? 2 : 1, PP = HM ? 1 : 2;    // pieces of a query and of a weight
     constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, U = DIM / 32, KB = DIM / 4 * BITS / 8, KW = KB / 4;
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
 
     // the row's position, and which drafts it sees
     int pos = rg.before + t; uint64_t seen = 0; int depth = 0;
-    if (a.parents) {
+    if (!ONE && a.parents) {
         const uint64_t all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
         depth = __popcll(all) - 1;                            // of draft `lane`
         seen = (uint64_t)__shfl((uint32_t)(all >> 32), t) << 32 | __shfl((uint32_t)all, t);
@@ -86,11 +86,14 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
         }
     }
 
+    // A wave asks for the next tile's keys when it has used this one's, for its values likewise, and for slots a tile earlier still: one set of registers for each, so that more waves
+    // than with two sets have a tile on its way.
     uint32_t kn[2][KW], vn[8][GROUPS][VW]; uint32_t ksn[2][NB], vsn[8][GROUPS];
-    auto request = [&](int c) {
-        const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept);
-        auto key = [&](int k) { const int j = j0 + k; return j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1); };      // keys no row sees give way to one that is seen
-        const int s = (int)kv_slot(a.p, table, (uint32_t)key(lane & 31));
+    auto slots_of = [&](int c) {
+        const int j = (c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept)) + (lane & 31);
+        return (int)kv_slot(a.p, table, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1)));      // keys no row sees give way to one that is seen
+    };
+    auto request_k = [&](int s) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const size_t sl = (uint32_t)__shfl(s, b * 16 + row);
@@ -102,6 +105,8 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
                 for (int i = 0; i < NB; i++) ksn[b][i] = sp[min(b0 + i, DIM / 32 - 1)];
             }
         }
+    };
+    auto request_v = [&](int s) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const size_t sl = (uint32_t)__shfl(s, (i >> 2) * 16 + 4 * q + (i & 3));
@@ -120,9 +125,16 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
     kv_f4 acc[DIM / 16];
 #pragma unroll
     for (int j = 0; j < DIM / 16; j++) acc[j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (c0 + wave < c1) request(c0 + wave);
+    int next = 0;
+    if (c0 + wave < c1) {
+        const int s = slots_of(c0 + wave);
+        if (c0 + wave + KVS_WAVES < c1) next = slots_of(c0 + wave + KVS_WAVES);
+        request_k(s); request_v(s);
+    }
     for (int c = c0 + wave; c < c1; c += KVS_WAVES) {
         const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept), end = c < rg.kept ? min(a.first, rg.hi) : rg.hi;
+        const int coming = next;
+        if (c + 2 * KVS_WAVES < c1) next = slots_of(c + 2 * KVS_WAVES);
         kv_f4 st[2];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -141,16 +153,9 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
                 for (int p = QP - 1; p >= 0; p--) st[b] = kvs_mfma<HM>(kf, qf[p][i], st[b]);
             }
         }
-        uint32_t vv[8][GROUPS][C / 2];
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int g = 0; g < GROUPS; g++) {
-                const float s = scaled ? kv_scale(vsn[i][g]) : 1.0f;
-#pragma unroll
-                for (int e = 0; e < C / 2; e++) vv[i][g][e] = kvs_two<FMT>(vn[i][g], e, s);
-            }
-        if (c + KVS_WAVES < c1) request(c + KVS_WAVES);
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + KVS_WAVES < c1) request_k(coming);
+        __builtin_amdgcn_sched_barrier(0);
         float cm = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
             for (int i = 0; i < 4; i++) {
                 const int key = j0 + b * 16 + 4 * q + i;
                 int at = key; bool ok = key < end;
-                if (a.parents) {
+                if (!ONE && a.parents) {
                     const int n = key - rg.before, d = __shfl(depth, n & 63);
                     if (n >= 0) { at = rg.before + d; ok = ok && (seen >> (n & 63) & 1); }
                 } else ok = ok && key <= pos;
@@ -180,53 +185,60 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
             if constexpr (PP == 2) pf[1][e] = kv_rest(p0, p1, pf[0][e]);
             vis[e] = (s0 == -INFINITY ? 0u : (HM ? 0x3C00u : 0x3F80u)) | (s1 == -INFINITY ? 0u : (HM ? 0x3C000000u : 0x3F800000u));
         }
-        constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, ONE = HM ? 0x3C00u : 0x3F80u;
+#pragma unroll
+        for (int j = 0; j < DIM / 16; j++) acc[j] *= alpha;
+        constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;
         // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys: nothing to do, but for an
         // infinity (16-bit pages hold them) and a weight whose second piece is 0 or negative.
-        bool odd = false;
-        if (it.cnt > 1 || (FMT == 0 && PP == 2)) {
+        const bool look = (FMT == 0 && PP == 2) || (!ONE && it.cnt > 1);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+        for (int g = 0; g < GROUPS; g++)
 #pragma unroll
-                for (int g = 0; g < GROUPS; g++)
+            for (int e2 = 0; e2 < C / 2; e2++) {
+                uint32_t w[8];
 #pragma unroll
-                    for (int e = 0; e < C / 2; e++) odd = odd || (vv[i][g][e] & EXP) == EXP || (vv[i][g][e] >> 16 & EXP) == EXP;
-            odd = __any(odd);
-        }
+                for (int i = 0; i < 8; i++) w[i] = kvs_two<FMT>(vn[i][g], e2, scaled ? kv_scale(vsn[i][g]) : 1.0f);
+                bool odd = false;
+                if (look) {
 #pragma unroll
-        for (int j = 0; j < DIM / 16; j++) {
-            u32x4 vf;
-#pragma unroll
-            for (int e = 0; e < 4; e++) vf[e] = __builtin_amdgcn_perm(vv[2 * e + 1][j / C][j % C / 2], vv[2 * e][j / C][j % C / 2], (j & 1) ? 0x07060302u : 0x05040100u);
-            acc[j] *= alpha;
-            if (odd) {                                        // such values apart: how many of them a row sees, by kind
-                u32x4 kind[3];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint32_t keep = 0; kind[0][e] = kind[1][e] = kind[2][e] = 0;
-#pragma unroll
-                    for (int h = 0; h < 32; h += 16) {
-                        const uint32_t x = vf[e] >> h & 0xFFFFu;
-                        if ((x & EXP) != EXP) keep |= x << h;
-                        else if (x & (HM ? 0x3FFu : 0x7Fu)) kind[2][e] |= ONE << h;
-                        else if (x & 0x8000u) kind[1][e] |= ONE << h;
-                        else kind[0][e] |= ONE << h;
-                    }
-                    vf[e] = keep;
+                    for (int i = 0; i < 8; i++) odd = odd || (w[i] & EXP) == EXP || (w[i] >> 16 & EXP) == EXP;
+                    odd = __any(odd);
                 }
-                const u32x4 see = {vis[0], vis[1], vis[2], vis[3]};
-                const kv_f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                const kv_f4 up = kvs_mfma<HM>(kind[0], see, zero), down = kvs_mfma<HM>(kind[1], see, zero), nan = kvs_mfma<HM>(kind[2], see, zero);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (up[i] > 0.0f) acc[j][i] += INFINITY;
-                    if (down[i] > 0.0f) acc[j][i] -= INFINITY;
-                    if (nan[i] > 0.0f) acc[j][i] = NAN;
+                for (int u = 0; u < 2; u++) {
+                    const int j = g * C + 2 * e2 + u;
+                    u32x4 vf;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) vf[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], u ? 0x07060302u : 0x05040100u);
+                    if (odd) {                                // such values apart: whether a row sees one, by kind
+                        const u32x4 see = {vis[0], vis[1], vis[2], vis[3]};
+                        u32x4 keep = vf;
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            u32x4 kind;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                kind[e] = 0;
+#pragma unroll
+                                for (int h = 0; h < 32; h += 16) {
+                                    const uint32_t x = vf[e] >> h & 0xFFFFu, t = (x & EXP) != EXP ? 3u : (x & (HM ? 0x3FFu : 0x7Fu)) ? 2u : x >> 15;
+                                    if (t == (uint32_t)k) kind[e] |= UNIT << h;
+                                    if (t != 3u) keep[e] &= ~(0xFFFFu << h);
+                                }
+                            }
+                            const kv_f4 n = kvs_mfma<HM>(kind, see, kv_f4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                            for (int i = 0; i < 4; i++) if (n[i] > 0.0f) acc[j][i] += k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
+                        }
+                        vf = keep;
+                    }
+#pragma unroll
+                    for (int p = PP - 1; p >= 0; p--) acc[j] = kvs_mfma<HM>(vf, pf[p], acc[j]);
                 }
             }
-#pragma unroll
-            for (int p = PP - 1; p >= 0; p--) acc[j] = kvs_mfma<HM>(vf, pf[p], acc[j]);
-        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + KVS_WAVES < c1) request_v(coming);
+        __builtin_amdgcn_sched_barrier(0);
     }
     // ---- the waves' states meet: [waves][16][DIM + 4] sums | [waves][16] maxima | [waves][16] denominators | [16] maximum | [16] denominator
     constexpr int VS = DIM + 4;
@@ -271,13 +283,15 @@ __global__ void __launch_bounds__(64 * KVS_WAVES) kr_kv_step_kernel(const KvAttn
     }
 }
 
-template <int DIM, int FMT> static int kvs_launch(const KvAttnArgs& a, int half, hipStream_t st) {
+template <int DIM, int FMT, bool HQ, bool ONE> static int kvs_launch(const KvAttnArgs& a, hipStream_t st) {
     const size_t lds = kvs_lds(DIM);
-    const void* fn = half ? (const void*)kr_kv_step_kernel<DIM, FMT, true> : (const void*)kr_kv_step_kernel<DIM, FMT, false>;
-    if (lds > 65536 && kr_lds_optin(fn, lds)) return 1;
-    if (half) hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, true>), dim3(a.items), dim3(64 * KVS_WAVES), lds, st, a);
-    else hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, false>), dim3(a.items), dim3(64 * KVS_WAVES), lds, st, a);
+    if (lds > 65536 && kr_lds_optin((const void*)kr_kv_step_kernel<DIM, FMT, HQ, ONE>, lds)) return 1;
+    hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, HQ, ONE>), dim3(a.items), dim3(64 * KVS_WAVES), lds, st, a);
     return 0;
+}
+template <int DIM, int FMT> static int kvs_launch(const KvAttnArgs& a, int half, hipStream_t st) {
+    if (a.one) return half ? kvs_launch<DIM, FMT, true, true>(a, st) : kvs_launch<DIM, FMT, false, true>(a, st);
+    return half ? kvs_launch<DIM, FMT, true, false>(a, st) : kvs_launch<DIM, FMT, false, false>(a, st);
 }
 template <int FMT> static int kvs_dim(const KvAttnArgs& a, int dim, int half, hipStream_t st) {
     switch (dim) {
@@ -293,36 +307,89 @@ int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream
     return fmt == 0 ? kvs_dim<0>(a, dim, half, st) : fmt == 1 ? kvs_dim<1>(a, dim, half, st) : kvs_dim<2>(a, dim, half, st);
 }
 
-// Shares of split sequences joined: unit = 16 rows of a row tile of bm rows and one head; a thread holds four columns of a row.
-template <bool H> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
-    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, bm / 16);
+// Shares of split sequences joined.  FEW (four shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares.  Else a unit is
+// one row: its threads divide the shares among themselves and meet in LDS.
+template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
+    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, FEW ? bm / 16 : bm);
     if (it.b < 0) return;
-    const int rows = it.cnt * a.G, quads = dim / 4;
+    const int rows = it.cnt * a.G, quads = dim / 4, tid = threadIdx.x, first = kv_item_of(a, it, bm, 0), step = a.kv_heads;      // a row tile's shares lie kv_heads items apart
     const float* stats = a.ws + (size_t)a.items * bm * dim;
-    for (int i = threadIdx.x; i < 16 * quads; i += 256) {
-        const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
-        if (rr >= rows) continue;
-        float top = -INFINITY;
-        for (int s = 0; s < it.nsplit; s++) top = fmaxf(top, stats[((size_t)kv_item_of(a, it, bm, s) * bm + r) * 2]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
-#pragma unroll 4
-        for (int s = 0; s < it.nsplit; s++) {
-            const size_t at = (size_t)kv_item_of(a, it, bm, s) * bm + r;
-            const float ms = stats[at * 2], f = __builtin_amdgcn_exp2f(ms - base), ls = stats[at * 2 + 1];
-            const float4 x = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
-            if (ms == -INFINITY && ls == 0.0f) continue;      // a share without keys of this row
-            o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
-            den += ls * f;
+    if constexpr (FEW) {
+        for (int i = tid; i < 16 * quads; i += 256) {
+            const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
+            if (rr >= rows) continue;
+            float ms[4], ls[4]; float4 x[4];
+            float top = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const size_t at = (size_t)(first + min(s, it.nsplit - 1) * step) * bm + r;
+                ms[s] = stats[at * 2]; ls[s] = stats[at * 2 + 1]; x[s] = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
+                top = fmaxf(top, ms[s]);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                if (s >= it.nsplit || (ms[s] == -INFINITY && ls[s] == 0.0f)) continue;      // a share without keys of this row
+                const float f = __builtin_amdgcn_exp2f(ms[s] - base);
+                o.x += x[s].x * f; o.y += x[s].y * f; o.z += x[s].z * f; o.w += x[s].w * f;
+                den += ls[s] * f;
+            }
+            const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+            const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
+            *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
         }
+    } else {
+        __shared__ float wl[KV_MAX_SHARES]; __shared__ float red[8]; __shared__ float4 sums[256];
+        const int r = it.split, rr = it.rt * bm + r;
+        if (rr >= rows) return;
+        float top = -INFINITY, den = 0.0f;
+        for (int s = tid; s < it.nsplit; s += 256) { const float ms = stats[((size_t)(first + s * step) * bm + r) * 2]; wl[s] = ms; top = fmaxf(top, ms); }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        if ((tid & 63) == 0) red[tid >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (int s = tid; s < it.nsplit; s += 256) {
+            const float ms = wl[s], ls = stats[((size_t)(first + s * step) * bm + r) * 2 + 1];
+            const bool none = ms == -INFINITY && ls == 0.0f;
+            const float f = none ? -1.0f : __builtin_amdgcn_exp2f(ms - base);      // -1: a share without keys of this row
+            wl[s] = f;
+            if (!none) den += ls * f;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) den += __shfl_xor(den, d);
+        if ((tid & 63) == 0) red[4 + (tid >> 6)] = den;
+        __syncthreads();
+        den = red[4] + red[5] + red[6] + red[7];
+        const int groups = 256 / quads, g = tid / quads, d = tid % quads * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (g < groups) {
+            const float* wp = a.ws + ((size_t)first * bm + r) * dim + d;
+#pragma unroll 4
+            for (int s = g; s < it.nsplit; s += groups) {
+                const float f = wl[s];
+                const float4 x = *reinterpret_cast<const float4*>(wp + (size_t)s * step * bm * dim);
+                if (f != -1.0f) { o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f; }
+            }
+        }
+        sums[tid] = o;
+        __syncthreads();
+        if (tid >= quads) return;
+        for (int k = 1; k < groups; k++) { const float4 x = sums[k * quads + tid]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
         const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
-        u32x2 w = {kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
-        *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = w;
+        *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
     }
 }
-int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int half, hipStream_t st) {
-    if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-    else hipLaunchKernelGGL((kr_kv_join_kernel<false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st) {
+    if (few) {
+        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+        else hipLaunchKernelGGL((kr_kv_join_kernel<false, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+    } else {
+        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+        else hipLaunchKernelGGL((kr_kv_join_kernel<false, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+    }
     return 0;
 }
