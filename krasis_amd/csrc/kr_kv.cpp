@@ -1,6 +1,7 @@
 // kr_kv.cpp -- entry points of the operators over a caller's paged cache: checks of arguments, the plan of a step, the division of attention into workgroups.
 #include <math.h>
 
+#include <algorithm>
 #include <vector>
 
 #include "kr_engine_internal.h"
@@ -72,9 +73,10 @@ int rows_call(const char* what, const kr_kv_pages* p, const int* plan, const int
 
 // one launch's share of a call: the sequences whose rows (new tokens x heads of a group) lie in a range
 struct Part { int min_rows, max_rows, bm, kt, tps; int64_t items, units; int shares; bool split, few, one; };
-// How many key tiles a workgroup takes: `hold` workgroups are on the chip at once, so the launch lasts rounds * (tiles a workgroup + what it takes to begin and to end, `extra` tiles),
-// and the cheapest number of rounds up to four is taken (more items than that without any sharing out: they fill the chip evenly by themselves).
-void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int hold, int least, int extra, Part& p) {
+// How many key tiles a workgroup takes.  `hold` workgroups are on the chip at once and `side` tiles are worked on side by side in one, so a launch lasts rounds * (tiles / side + what it
+// takes to begin and to end, `extra`), and `join` more when shares have to be joined (all in the time of a tile); the cheapest number of rounds up to four is taken.  More row tiles than
+// that fill the chip evenly by themselves.
+void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int hold, int side, int extra, int join, Part& p) {
     struct Seq { int tiles; int64_t row_tiles; };
     std::vector<Seq> seqs;
     int64_t total = 0, whole = 0; int longest = 0;
@@ -89,14 +91,13 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
     p.items = whole; p.units = 0; p.split = p.few = false; p.one = !tree; p.tps = longest > 0 ? longest : 1;
     if (seqs.empty()) return;
     auto items = [&](int tps) { int64_t n = 0; for (const Seq& s : seqs) n += s.row_tiles * ((s.tiles + tps - 1) / tps); return n; };
-    if (whole < 4ll * hold && longest > least) {
-        int64_t best = ((whole + hold - 1) / hold) * (longest + extra);
+    if (whole < 4ll * hold) {
+        const int least = std::max(side, (longest + KV_MAX_SHARES - 1) / KV_MAX_SHARES);
+        int64_t best = ((whole + hold - 1) / hold) * ((longest + side - 1) / side + extra);
         for (int64_t k = (whole + hold - 1) / hold; k <= 4; k++) {
-            int lo = (int)(total / (k * hold)), hi = longest;      // the smallest share whose items fit into k rounds
-            if (lo < least) lo = least;
-            if (lo < (longest + KV_MAX_SHARES - 1) / KV_MAX_SHARES) lo = (longest + KV_MAX_SHARES - 1) / KV_MAX_SHARES;
+            int lo = std::max(least, (int)(total / (k * hold))), hi = longest;      // the smallest share whose items fit into k rounds
             while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (items(mid) <= k * hold) hi = mid; else lo = mid + 1; }
-            const int64_t cost = k * (lo + extra);
+            const int64_t cost = k * ((lo + side - 1) / side + extra) + join;
             if (lo < longest && cost < best) { best = cost; p.tps = lo; }
         }
     }
@@ -109,15 +110,15 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
         most = ns > most ? ns : most;
     }
     p.shares = most;
-    p.few = most <= 4;
+    p.few = most <= 8;
     if (p.split) for (const Seq& s : seqs) if (s.tiles > p.tps) p.units += s.row_tiles * (p.few ? p.bm / 16 : p.bm);
 }
 void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, int window, int first, bool tree, Part* p) {
     const int G = heads / kv_heads;
     p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, 1, false, false, false};
     p[1] = Part{KV_STEP_BM + 1, INT32_MAX, KV_TILE_BM, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
-    divide(h, kv_heads, G, window, first, tree, kv_step_hold(dim, fmt) * KV_CUS, 4, 8, p[0]);
-    divide(h, kv_heads, G, window, first, tree, dim <= 128 ? 2 * KV_CUS : KV_CUS, 2, 3, p[1]);
+    divide(h, kv_heads, G, window, first, tree, KV_CUS, kv_step_waves(dim, fmt), 3, 3, p[0]);
+    divide(h, kv_heads, G, window, first, tree, dim <= 128 ? 2 * KV_CUS : KV_CUS, 1, 2, 4, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
 

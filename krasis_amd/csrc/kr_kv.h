@@ -49,7 +49,7 @@ constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 
 constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step.hip
 constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile.hip
-__host__ __device__ constexpr int kv_step_hold(int dim, int fmt) { return dim <= 128 ? 3 : dim == 256 && fmt == 0 ? 1 : 2; }      // workgroups of four waves a CU: by registers
+__host__ __device__ constexpr int kv_step_waves(int dim, int fmt) { return dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8; }      // of a workgroup in kr_kv_step.hip, one a CU: by registers
 constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
 
 // ---- the division of a launch into items, the same on the host (how many) and on the device (which one)

@@ -4,14 +4,13 @@
 // Keys and values go from the pages to registers once, converted there to bf16 (exact, kr_kv_dev.h), and meet the queries in v_mfma_f32_16x16x32:
 //   S^T[key][row] = K Q^T    first operand: 16 key rows; a lane holds a quarter of a row, so a microscaled row costs it one scale and loads of 16 bytes
 //   O^T[d][row] += V^T P^T   a lane holds 8 keys and c neighbouring columns; byte permutes make them the columns' fragments
-// A workgroup takes one sequence, one key / value head and a share of its key tiles; its four waves take tiles of 32 keys in turn, each with a running maximum and sum per row, and
+// A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a running maximum and sum per row, and
 // meet in LDS.  Weights are taken as two bf16 pieces (16 bits), f16 queries over bf16-converted pages too: the matrix cores have time for it here.
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
 
-constexpr int KVS_WAVES = 4;
 template <int DIM> struct KvsCols { static constexpr int C = DIM == 96 ? 2 : DIM == 192 ? 4 : DIM / 16, GROUPS = DIM / (16 * C); };      // columns of V a lane holds: groups of 16 C
-inline int kvs_lds(int dim) { return (KVS_WAVES * 16 * (dim + 4) + KVS_WAVES * 32 + 32) * (int)sizeof(float); }
+constexpr int kvs_lds(int dim, int waves) { return (waves * 16 * (dim + 4) + waves * 32 + 32) * (int)sizeof(float); }
 
 template <int BYTES> __device__ __forceinline__ void kvs_load(const uint8_t* p, uint32_t* w) {
     if constexpr (BYTES % 16 == 0) {
@@ -39,7 +38,8 @@ template <bool H> __device__ __forceinline__ kv_f4 kvs_mfma(u32x4 x, u32x4 y, kv
 
 // HQ: q and out are f16.  Products are f16 where the pages are f16 too, else bf16.  ONE: every sequence of the launch has one new token and no tree, so that its rows see the same keys.
 template <int DIM, int FMT, bool HQ, bool ONE>
-__global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_step_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DIM, FMT) / 4) kr_kv_step_kernel(const KvAttnArgs a) {
+    constexpr int WAVES = kv_step_waves(DIM, FMT);
     constexpr bool HM = HQ && FMT == 0;                       // f16 products
     constexpr int QP = HQ && !HM ? 2 : 1, PP = HM ? 1 : 2;    // pieces of a query and of a weight
     constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, U = DIM / 32, KB = DIM / 4 * BITS / 8, KW = KB / 4;
@@ -128,13 +128,13 @@ __global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_
     int next = 0;
     if (c0 + wave < c1) {
         const int s = slots_of(c0 + wave);
-        if (c0 + wave + KVS_WAVES < c1) next = slots_of(c0 + wave + KVS_WAVES);
+        if (c0 + wave + WAVES < c1) next = slots_of(c0 + wave + WAVES);
         request_k(s); request_v(s);
     }
-    for (int c = c0 + wave; c < c1; c += KVS_WAVES) {
+    for (int c = c0 + wave; c < c1; c += WAVES) {
         const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept), end = c < rg.kept ? min(a.first, rg.hi) : rg.hi;
         const int coming = next;
-        if (c + 2 * KVS_WAVES < c1) next = slots_of(c + 2 * KVS_WAVES);
+        if (c + 2 * WAVES < c1) next = slots_of(c + 2 * WAVES);
         kv_f4 st[2];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (c + KVS_WAVES < c1) request_k(coming);
+        if (c + WAVES < c1) request_k(coming);
         __builtin_amdgcn_sched_barrier(0);
         float cm = -INFINITY;
 #pragma unroll
@@ -237,21 +237,21 @@ __global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_
                 }
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (c + KVS_WAVES < c1) request_v(coming);
+        if (c + WAVES < c1) request_v(coming);
         __builtin_amdgcn_sched_barrier(0);
     }
     // ---- the waves' states meet: [waves][16][DIM + 4] sums | [waves][16] maxima | [waves][16] denominators | [16] maximum | [16] denominator
     constexpr int VS = DIM + 4;
-    float* ml = kvs_lds_ + KVS_WAVES * 16 * VS; float* dl = ml + KVS_WAVES * 16; float* mt = dl + KVS_WAVES * 16; float* dt = mt + 16;
+    float* ml = kvs_lds_ + WAVES * 16 * VS; float* dl = ml + WAVES * 16; float* mt = dl + WAVES * 16; float* dt = mt + 16;
     l += __shfl_xor(l, 16); l += __shfl_xor(l, 32);
     if (q == 0) { ml[wave * 16 + row] = m; dl[wave * 16 + row] = l; }
     __syncthreads();
     float top = -INFINITY, den = 0.0f;
 #pragma unroll
-    for (int w = 0; w < KVS_WAVES; w++) top = fmaxf(top, ml[w * 16 + row]);
+    for (int w = 0; w < WAVES; w++) top = fmaxf(top, ml[w * 16 + row]);
     const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-    for (int w = 0; w < KVS_WAVES; w++) den += dl[w * 16 + row] * __builtin_amdgcn_exp2f(ml[w * 16 + row] - base);
+    for (int w = 0; w < WAVES; w++) den += dl[w * 16 + row] * __builtin_amdgcn_exp2f(ml[w * 16 + row] - base);
     const float f = __builtin_amdgcn_exp2f(m - base);
     float* mine = kvs_lds_ + (wave * 16 + row) * VS;
 #pragma unroll
@@ -262,11 +262,11 @@ __global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_
     __syncthreads();
     const bool whole = it.nsplit == 1;
     float* wo = a.ws + (size_t)blockIdx.x * 16 * DIM;
-    for (int i = tid; i < rows * (DIM / 4); i += 64 * KVS_WAVES) {
+    for (int i = tid; i < rows * (DIM / 4); i += 64 * WAVES) {
         const int rr = i / (DIM / 4), d = (i - rr * (DIM / 4)) * 4;
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < KVS_WAVES; w++) {
+        for (int w = 0; w < WAVES; w++) {
             const float4 x = *reinterpret_cast<const float4*>(kvs_lds_ + (w * 16 + rr) * VS + d);
             s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
         }
@@ -284,9 +284,10 @@ __global__ void __launch_bounds__(64 * KVS_WAVES, kv_step_hold(DIM, FMT)) kr_kv_
 }
 
 template <int DIM, int FMT, bool HQ, bool ONE> static int kvs_launch(const KvAttnArgs& a, hipStream_t st) {
-    const size_t lds = kvs_lds(DIM);
+    constexpr int waves = kv_step_waves(DIM, FMT);
+    constexpr size_t lds = kvs_lds(DIM, waves);
     if (lds > 65536 && kr_lds_optin((const void*)kr_kv_step_kernel<DIM, FMT, HQ, ONE>, lds)) return 1;
-    hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, HQ, ONE>), dim3(a.items), dim3(64 * KVS_WAVES), lds, st, a);
+    hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, HQ, ONE>), dim3(a.items), dim3(64 * waves), lds, st, a);
     return 0;
 }
 template <int DIM, int FMT> static int kvs_launch(const KvAttnArgs& a, int half, hipStream_t st) {
@@ -307,7 +308,7 @@ int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream
     return fmt == 0 ? kvs_dim<0>(a, dim, half, st) : fmt == 1 ? kvs_dim<1>(a, dim, half, st) : kvs_dim<2>(a, dim, half, st);
 }
 
-// Shares of split sequences joined.  FEW (four shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares.  Else a unit is
+// Shares of split sequences joined.  FEW (eight shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares.  Else a unit is
 // one row: its threads divide the shares among themselves and meet in LDS.
 template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
     const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, FEW ? bm / 16 : bm);
@@ -318,10 +319,10 @@ template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_ke
         for (int i = tid; i < 16 * quads; i += 256) {
             const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
             if (rr >= rows) continue;
-            float ms[4], ls[4]; float4 x[4];
+            float ms[8], ls[8]; float4 x[8];
             float top = -INFINITY;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
+            for (int s = 0; s < 8; s++) {
                 const size_t at = (size_t)(first + min(s, it.nsplit - 1) * step) * bm + r;
                 ms[s] = stats[at * 2]; ls[s] = stats[at * 2 + 1]; x[s] = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
                 top = fmaxf(top, ms[s]);
@@ -329,7 +330,7 @@ template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_ke
             const float base = top == -INFINITY ? 0.0f : top;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
+            for (int s = 0; s < 8; s++) {
                 if (s >= it.nsplit || (ms[s] == -INFINITY && ls[s] == 0.0f)) continue;      // a share without keys of this row
                 const float f = __builtin_amdgcn_exp2f(ms[s] - base);
                 o.x += x[s].x * f; o.y += x[s].y * f; o.z += x[s].z * f; o.w += x[s].w * f;
