@@ -37,6 +37,10 @@ int check_pages(const kr_kv_pages* p, const int* plan, KvPages& o) {
     o.k = (uint8_t*)p->k; o.v = (uint8_t*)p->v; o.ks = (uint8_t*)p->k_scale; o.vs = (uint8_t*)p->v_scale;
     o.head_bytes = p->dim * bits_of(p->format) / 8; o.row_bytes = o.head_bytes * p->kv_heads;
     o.shead_bytes = scaled(p->format) ? p->dim / 32 : 0; o.srow_bytes = o.shead_bytes * p->kv_heads;
+    if (p->format == KR_KV_E4M3) { o.ks = o.k; o.vs = o.v; o.shead_bytes = o.head_bytes; o.srow_bytes = o.row_bytes; }      // read, and replaced by 127
+    if ((int64_t)p->page_tokens * p->n_pages * (o.row_bytes / 16) > UINT32_MAX) return kr_fail(KR_ERR_VALUE, "kr_kv: %d pages of %d tokens are more than 64 GiB", p->n_pages, p->page_tokens);
+    o.row16 = (uint32_t)o.row_bytes / 16; o.scale_and = scaled(p->format) ? 0xFFu : 0u; o.scale_or = scaled(p->format) ? 0u : 127u;
+    o.scale_shift = p->format == KR_KV_MX8 ? 1 : 0;
     o.page_tokens = p->page_tokens;
     o.page_magic = p->page_tokens == 1 ? 0xFFFFFFFFu : (uint32_t)((1ull << 32) / (uint64_t)p->page_tokens);
     return KR_OK;
@@ -113,12 +117,15 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
     p.few = most <= 8;
     if (p.split) for (const Seq& s : seqs) if (s.tiles > p.tps) p.units += s.row_tiles * (p.few ? p.bm / 16 : p.bm);
 }
-void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, int window, int first, bool tree, Part* p) {
+void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, int half, int window, int first, bool tree, Part* p) {
     const int G = heads / kv_heads;
     p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, 1, false, false, false};
-    p[1] = Part{KV_STEP_BM + 1, INT32_MAX, KV_TILE_BM, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
+    int64_t most = 0;
+    for (int b = 0; b < h.batch; b++) most = std::max(most, (int64_t)(h.row0[b + 1] - h.row0[b]) * G);
+    const int blocks = kv_tile_two(dim, fmt, half) && most > 128 ? 2 : 1;      // a second block of 32 rows a wave, where sequences have rows for it
+    p[1] = Part{KV_STEP_BM + 1, INT32_MAX, 128 * blocks, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
     divide(h, kv_heads, G, window, first, tree, KV_CUS, kv_step_waves(dim, fmt), 3, 3, p[0]);
-    divide(h, kv_heads, G, window, first, tree, dim <= 128 ? 2 * KV_CUS : KV_CUS, 1, 2, 4, p[1]);
+    divide(h, kv_heads, G, window, first, tree, kv_tile_waves(dim, blocks) * KV_CUS, 1, 3, 4, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
 
@@ -192,13 +199,13 @@ extern "C" int kr_kv_read(const kr_kv_pages* p, const int* plan, const int* dev_
     return rows_call("kr_kv_read", p, plan, dev_plan, k, v, strides, dtype, stream, false);
 }
 
-extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int window, int keep_first, int tree, size_t* bytes) {
+extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int dtype, int window, int keep_first, int tree, size_t* bytes) {
     KvPages o;
     if (int rc = check_attend(p, plan, heads, window, keep_first, tree != 0, o)) return rc;
     if (!bytes) return kr_fail(KR_ERR_VALUE, "kr_kv_attend_workspace: null argument");
     const Plan h(plan);
     Part part[2];
-    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), window, clamp_first(h, window, keep_first), tree != 0, part);
+    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), dtype == KR_KV_F16, window, clamp_first(h, window, keep_first), tree != 0, part);
     *bytes = part_bytes(part[0], p->dim) + part_bytes(part[1], p->dim);
     return KR_OK;
 }
@@ -220,17 +227,19 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
     a.window = window; a.first = clamp_first(h, window, keep_first);
     a.scale_log2 = scale * 1.44269504088896340736f;
     Part part[2];
-    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), window, a.first, parents != nullptr, part);
+    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), dtype == KR_KV_F16, window, a.first, parents != nullptr, part);
     const size_t b0 = part_bytes(part[0], p->dim), b1 = part_bytes(part[1], p->dim);
     if (workspace_bytes < b0 + b1 || ((b0 + b1) && (!workspace || misaligned(workspace)))) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: a workspace of %zu bytes for %zu", workspace_bytes, b0 + b1);
     if (part[0].items > INT32_MAX || part[1].items > INT32_MAX || part[0].units > INT32_MAX || part[0].shares > KV_MAX_SHARES || part[1].shares > KV_MAX_SHARES || part[1].units > INT32_MAX) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: %d rows are too many for one call", h.rows);
     const int fmt = fmt_of(p->format), half = dtype == KR_KV_F16;
     hipStream_t st = stream_of(stream);
+    static int (*const step[3])(const KvAttnArgs&, int, int, hipStream_t) = {kr_launch_kv_step_16, kr_launch_kv_step_8, kr_launch_kv_step_4};
+    static int (*const tile[3])(const KvAttnArgs&, int, int, int, hipStream_t) = {kr_launch_kv_tile_16, kr_launch_kv_tile_8, kr_launch_kv_tile_4};
     for (int i = 1; i >= 0; i--) {                            // prompts first, they take longest
         if (!part[i].items) continue;
         a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = part[i].tps; a.items = (int)part[i].items; a.one = part[i].one;
         a.ws = (float*)((char*)workspace + (i ? b0 : 0));
-        if (int rc = launched("kr_kv_attend", i ? kr_launch_kv_tile(a, p->dim, fmt, half, st) : kr_launch_kv_step(a, p->dim, fmt, half, st))) return rc;
+        if (int rc = launched("kr_kv_attend", i ? tile[fmt](a, p->dim, half, part[i].bm / 128, st) : step[fmt](a, p->dim, half, st))) return rc;
         if (part[i].split)
             if (int rc = launched("kr_kv_attend", kr_launch_kv_join(a, p->dim, part[i].bm, part[i].kt, (int)part[i].units, part[i].few, half, st))) return rc;
     }
@@ -246,8 +255,8 @@ extern "C" int kr_kv_move(const kr_kv_pages* p, int layers, int n_seq, const int
     if (!dev_start || !dev_src || !dev_dst) return kr_fail(KR_ERR_VALUE, "kr_kv_move: null argument");
     KvMoveArgs a{};
     const int64_t slots = (int64_t)p->n_pages * p->page_tokens;
-    a.base[0] = o.k; a.base[1] = o.v; a.base[2] = o.ks; a.base[3] = o.vs;
-    for (int i = 0; i < 4; i++) { a.row_bytes[i] = i < 2 ? o.row_bytes : o.srow_bytes; a.layer_bytes[i] = slots * a.row_bytes[i]; }
+    a.base[0] = o.k; a.base[1] = o.v; a.base[2] = (uint8_t*)p->k_scale; a.base[3] = (uint8_t*)p->v_scale;
+    for (int i = 0; i < 4; i++) { a.row_bytes[i] = i < 2 ? o.row_bytes : scaled(p->format) ? o.srow_bytes : 0; a.layer_bytes[i] = slots * a.row_bytes[i]; }
     a.start = dev_start; a.src = dev_src; a.dst = dev_dst; a.n_seq = n_seq; a.layers = layers;
     return launched("kr_kv_move", kr_launch_kv_move(a, stream_of(stream)));
 }

@@ -1,5 +1,5 @@
 // kr_kv.h -- operators over a caller's paged key / value cache (krasis_amd.kv_cache.PagedKVCache): what the entry points in kr_kv.cpp hand to the kernels in kr_kv_store.hip
-// (rows quantised into the pages, read back, moved), kr_kv_step.hip and kr_kv_tile.hip (attention over the pages).
+// (rows quantised into the pages, read back, moved), kr_kv_step_dev.h and kr_kv_tile_dev.h (attention over the pages) and kr_kv_join.hip.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -11,6 +11,9 @@ struct KvPages {
     uint8_t *k, *v, *ks, *vs;
     int row_bytes, srow_bytes;         // bytes of a slot: all heads' codes / scales
     int head_bytes, shead_bytes;       // bytes of one head of a slot
+    uint32_t row16;                    // row_bytes / 16: places in the pages are counted in units of 16 bytes
+    uint32_t scale_and, scale_or;      // (scale byte & scale_and) | scale_or: pages of plain E4M3 give any byte of theirs, which becomes 127
+    int scale_shift;                   // place in the pages >> scale_shift = place of its scales
     int page_tokens;
     uint32_t page_magic;               // floor(2^32 / page_tokens), at most 2^32 - 1: kv_page() below
 };
@@ -41,15 +44,21 @@ struct KvAttnArgs {
 int kr_launch_kv_write(const KvRowsArgs& a, hipStream_t st);
 int kr_launch_kv_read(const KvRowsArgs& a, hipStream_t st);
 int kr_launch_kv_move(const KvMoveArgs& a, hipStream_t st);
-// fmt: 0 16-bit pages, 1 eight bits, 2 four bits; half: q and out are f16
-int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st);
-int kr_launch_kv_tile(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st);
+// by the width of the pages' numbers; half: q and out are f16; blocks: of 32 rows a wave
+int kr_launch_kv_step_16(const KvAttnArgs& a, int dim, int half, hipStream_t st);
+int kr_launch_kv_step_8(const KvAttnArgs& a, int dim, int half, hipStream_t st);
+int kr_launch_kv_step_4(const KvAttnArgs& a, int dim, int half, hipStream_t st);
+int kr_launch_kv_tile_16(const KvAttnArgs& a, int dim, int half, int blocks, hipStream_t st);
+int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, int blocks, hipStream_t st);
+int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, int blocks, hipStream_t st);
 int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st);
 constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 
-constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step.hip
-constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile.hip
-__host__ __device__ constexpr int kv_step_waves(int dim, int fmt) { return dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8; }      // of a workgroup in kr_kv_step.hip, one a CU: by registers
+constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step_dev.h
+constexpr int KV_TILE_KT = 64;       // keys of a tile in kr_kv_tile_dev.h, whose workgroups take 128 rows a block
+__host__ __device__ constexpr bool kv_tile_two(int dim, int fmt, int half) { return dim <= 128 && (!half || fmt == 0); }      // two blocks of 32 rows fit a wave's registers
+__host__ __device__ constexpr int kv_tile_waves(int dim, int blocks) { return dim <= 128 && blocks == 1 ? 2 : 1; }           // waves a SIMD holds
+__host__ __device__ constexpr int kv_step_waves(int dim, int fmt) { return dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8; }      // of a workgroup in kr_kv_step_dev.h, one a CU: by registers
 constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
 
 // ---- the division of a launch into items, the same on the host (how many) and on the device (which one)

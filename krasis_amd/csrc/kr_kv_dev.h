@@ -24,12 +24,13 @@ __device__ __forceinline__ uint32_t kv_slot(const KvPages& p, const int* table, 
 }
 
 // two neighbouring codes of a dword times the scale as a packed pair of bf16.  E4M3 and E2M1 have at most four significant bits and scales are powers of two of at least 2^-100:
-// every product is exact in bf16.  A scale byte of 255 stands for a block that held a NaN or an infinity and reads back as NaN.
+// every product is exact in bf16.
 template <int FMT, int SEL> __device__ __forceinline__ uint32_t kv_pair(uint32_t w, float scale) {
     if constexpr (FMT == 1) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, SEL != 0));
     else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
 }
-__device__ __forceinline__ float kv_scale(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7FC00000u : byte << 23); }
+// the conversions take the scale's exponent field, of which 255 is NaN for any code (measured): the byte needs no case of its own
+__device__ __forceinline__ float kv_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 template <bool H> __device__ __forceinline__ uint32_t kv_pack(float a, float b) {      // round to nearest even
     if constexpr (H) { kv_h2 x; x[0] = (_Float16)a; x[1] = (_Float16)b; return __builtin_bit_cast(uint32_t, x); }

@@ -1,0 +1,89 @@
+// kr_kv_join.hip -- the second launch of attention over the paged cache, where sequences were shared out among workgroups.
+#include "kr_kv_dev.h"
+
+// Shares of split sequences joined.  FEW (eight shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares.  Else a unit is
+// one row: its threads divide the shares among themselves and meet in LDS.
+template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
+    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, FEW ? bm / 16 : bm);
+    if (it.b < 0) return;
+    const int rows = it.cnt * a.G, quads = dim / 4, tid = threadIdx.x, first = kv_item_of(a, it, bm, 0), step = a.kv_heads;      // a row tile's shares lie kv_heads items apart
+    const float* stats = a.ws + (size_t)a.items * bm * dim;
+    if constexpr (FEW) {
+        for (int i = tid; i < 16 * quads; i += 256) {
+            const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
+            if (rr >= rows) continue;
+            float ms[8], ls[8]; float4 x[8];
+            float top = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const size_t at = (size_t)(first + min(s, it.nsplit - 1) * step) * bm + r;
+                ms[s] = stats[at * 2]; ls[s] = stats[at * 2 + 1]; x[s] = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
+                top = fmaxf(top, ms[s]);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                if (s >= it.nsplit || (ms[s] == -INFINITY && ls[s] == 0.0f)) continue;      // a share without keys of this row
+                const float f = __builtin_amdgcn_exp2f(ms[s] - base);
+                o.x += x[s].x * f; o.y += x[s].y * f; o.z += x[s].z * f; o.w += x[s].w * f;
+                den += ls[s] * f;
+            }
+            const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+            const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
+            *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
+        }
+    } else {
+        __shared__ float wl[KV_MAX_SHARES]; __shared__ float red[8]; __shared__ float4 sums[256];
+        const int r = it.split, rr = it.rt * bm + r;
+        if (rr >= rows) return;
+        float top = -INFINITY, den = 0.0f;
+        for (int s = tid; s < it.nsplit; s += 256) { const float ms = stats[((size_t)(first + s * step) * bm + r) * 2]; wl[s] = ms; top = fmaxf(top, ms); }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        if ((tid & 63) == 0) red[tid >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (int s = tid; s < it.nsplit; s += 256) {
+            const float ms = wl[s], ls = stats[((size_t)(first + s * step) * bm + r) * 2 + 1];
+            const bool none = ms == -INFINITY && ls == 0.0f;
+            const float f = none ? -1.0f : __builtin_amdgcn_exp2f(ms - base);      // -1: a share without keys of this row
+            wl[s] = f;
+            if (!none) den += ls * f;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) den += __shfl_xor(den, d);
+        if ((tid & 63) == 0) red[4 + (tid >> 6)] = den;
+        __syncthreads();
+        den = red[4] + red[5] + red[6] + red[7];
+        const int groups = 256 / quads, g = tid / quads, d = tid % quads * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (g < groups) {
+            const float* wp = a.ws + ((size_t)first * bm + r) * dim + d;
+#pragma unroll 4
+            for (int s = g; s < it.nsplit; s += groups) {
+                const float f = wl[s];
+                const float4 x = *reinterpret_cast<const float4*>(wp + (size_t)s * step * bm * dim);
+                if (f != -1.0f) { o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f; }
+            }
+        }
+        sums[tid] = o;
+        __syncthreads();
+        if (tid >= quads) return;
+        for (int k = 1; k < groups; k++) { const float4 x = sums[k * quads + tid]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
+        *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
+    }
+}
+int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st) {
+    if (few) {
+        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+        else hipLaunchKernelGGL((kr_kv_join_kernel<false, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+    } else {
+        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+        else hipLaunchKernelGGL((kr_kv_join_kernel<false, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+    }
+    return 0;
+}

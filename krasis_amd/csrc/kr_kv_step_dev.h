@@ -1,4 +1,4 @@
-// kr_kv_step.hip -- attention over the paged cache for sequences with at most 16 rows of new tokens (one token of a group of up to 16 heads, a few tokens of smaller groups):
+// kr_kv_step_dev.h -- attention over the paged cache for sequences with at most 16 rows of new tokens (one token of a group of up to 16 heads, a few tokens of smaller groups):
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the stored keys j that row i sees.
 // A row of keys serves 16 rows of queries: 4 * 16 operations a channel against one to four bytes of it, far under the matrix rate, so the launch is bound by HBM and its latency.
 // Keys and values go from the pages to registers once, converted there to bf16 (exact, kr_kv_dev.h), and meet the queries in v_mfma_f32_16x16x32:
@@ -6,6 +6,7 @@
 //   O^T[d][row] += V^T P^T   a lane holds 8 keys and c neighbouring columns; byte permutes make them the columns' fragments
 // A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a running maximum and sum per row, and
 // meet in LDS.  Weights are taken as two bf16 pieces (16 bits), f16 queries over bf16-converted pages too: the matrix cores have time for it here.
+#pragma once
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
 
@@ -53,11 +54,10 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     const int c0 = it.split * a.tps, c1 = min(rg.tiles, c0 + a.tps);
     const int rows = it.cnt * a.G, r = min(row, rows - 1), t = r / a.G, head = it.kvh * a.G + r - t * a.G;
     const int* table = a.s.pages + it.page0;
-    const bool scaled = FMT != 0 && a.p.ks != nullptr;
     const uint8_t* kbase = a.p.k + (size_t)it.kvh * a.p.head_bytes + q * KB;
     const uint8_t* vbase = a.p.v + (size_t)it.kvh * a.p.head_bytes;
-    const uint8_t* ksb = a.p.ks + (size_t)it.kvh * a.p.shead_bytes;
-    const uint8_t* vsb = a.p.vs + (size_t)it.kvh * a.p.shead_bytes;
+    const uint8_t* ksb = a.p.ks + it.kvh * a.p.shead_bytes; const uint8_t* vsb = a.p.vs + it.kvh * a.p.shead_bytes;
+    auto scale_of = [&](uint32_t byte) { return kv_scale((byte & a.p.scale_and) | a.p.scale_or); };
 
     // the row's position, and which drafts it sees
     int pos = rg.before + t; uint64_t seen = 0; int depth = 0;
@@ -89,34 +89,34 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     // A wave asks for the next tile's keys when it has used this one's, for its values likewise, and for slots a tile earlier still: one set of registers for each, so that more waves
     // than with two sets have a tile on its way.
     uint32_t kn[2][KW], vn[8][GROUPS][VW]; uint32_t ksn[2][NB], vsn[8][GROUPS];
-    auto slots_of = [&](int c) {
+    auto places = [&](int c) {                                // of key `lane` of a tile, in units of 16 bytes; keys no row sees give way to one that is seen
         const int j = (c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept)) + (lane & 31);
-        return (int)kv_slot(a.p, table, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1)));      // keys no row sees give way to one that is seen
+        return kv_slot(a.p, table, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1))) * a.p.row16;
     };
-    auto request_k = [&](int s) {
+    auto request_k = [&](uint32_t s) {
+        uint32_t at[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) at[b] = __shfl(s, b * 16 + row);
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const size_t sl = (uint32_t)__shfl(s, b * 16 + row);
-            kvs_load<KB>(kbase + sl * a.p.row_bytes, kn[b]);
-            if (scaled) {
-                const uint8_t* sp = ksb + sl * a.p.srow_bytes;
-                const int b0 = (q * U) >> 2;
+            kvs_load<KB>(kbase + ((uint64_t)at[b] << 4), kn[b]);
+            if constexpr (FMT != 0) {
+                const uint32_t b0 = (uint32_t)(q * U) >> 2;
 #pragma unroll
-                for (int i = 0; i < NB; i++) ksn[b][i] = sp[min(b0 + i, DIM / 32 - 1)];
+                for (int i = 0; i < NB; i++) ksn[b][i] = ksb[(at[b] >> a.p.scale_shift) + min(b0 + i, (uint32_t)DIM / 32 - 1)];
             }
         }
     };
-    auto request_v = [&](int s) {
+    auto request_v = [&](uint32_t s) {
+        uint32_t at[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) at[i] = __shfl(s, (i >> 2) * 16 + 4 * q + (i & 3));
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const size_t sl = (uint32_t)__shfl(s, (i >> 2) * 16 + 4 * q + (i & 3));
-            const uint8_t* vp = vbase + sl * a.p.row_bytes + row * VB;
 #pragma unroll
-            for (int g = 0; g < GROUPS; g++) kvs_load<VB>(vp + g * 16 * VB, vn[i][g]);
-            if (scaled) {
-                const uint8_t* sp = vsb + sl * a.p.srow_bytes;
-#pragma unroll
-                for (int g = 0; g < GROUPS; g++) vsn[i][g] = sp[(g * 16 * C + row * C) / 32];
+            for (int g = 0; g < GROUPS; g++) {
+                kvs_load<VB>(vbase + row * VB + g * 16 * VB + ((uint64_t)at[i] << 4), vn[i][g]);
+                if constexpr (FMT != 0) vsn[i][g] = vsb[(at[i] >> a.p.scale_shift) + (uint32_t)(g * 16 * C + row * C) / 32];
             }
         }
     };
@@ -125,23 +125,23 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     kv_f4 acc[DIM / 16];
 #pragma unroll
     for (int j = 0; j < DIM / 16; j++) acc[j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    int next = 0;
+    uint32_t next = 0;
     if (c0 + wave < c1) {
-        const int s = slots_of(c0 + wave);
-        if (c0 + wave + WAVES < c1) next = slots_of(c0 + wave + WAVES);
+        const uint32_t s = places(c0 + wave);
+        if (c0 + wave + WAVES < c1) next = places(c0 + wave + WAVES);
         request_k(s); request_v(s);
     }
     for (int c = c0 + wave; c < c1; c += WAVES) {
         const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept), end = c < rg.kept ? min(a.first, rg.hi) : rg.hi;
-        const int coming = next;
-        if (c + 2 * WAVES < c1) next = slots_of(c + 2 * WAVES);
+        const uint32_t coming = next;
+        if (c + 2 * WAVES < c1) next = places(c + 2 * WAVES);
         kv_f4 st[2];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             st[b] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
             float sc[NB];
 #pragma unroll
-            for (int i = 0; i < NB; i++) sc[i] = scaled ? kv_scale(ksn[b][i]) : 1.0f;
+            for (int i = 0; i < NB; i++) sc[i] = FMT == 0 ? 1.0f : scale_of(ksn[b][i]);
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 float s = sc[0];
@@ -185,8 +185,10 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
             if constexpr (PP == 2) pf[1][e] = kv_rest(p0, p1, pf[0][e]);
             vis[e] = (s0 == -INFINITY ? 0u : (HM ? 0x3C00u : 0x3F80u)) | (s1 == -INFINITY ? 0u : (HM ? 0x3C000000u : 0x3F800000u));
         }
+        if (__any(alpha != 1.0f)) {
 #pragma unroll
-        for (int j = 0; j < DIM / 16; j++) acc[j] *= alpha;
+            for (int j = 0; j < DIM / 16; j++) acc[j] *= alpha;
+        }
         constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;
         // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys: nothing to do, but for an
         // infinity (16-bit pages hold them) and a weight whose second piece is 0 or negative.
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
             for (int e2 = 0; e2 < C / 2; e2++) {
                 uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = kvs_two<FMT>(vn[i][g], e2, scaled ? kv_scale(vsn[i][g]) : 1.0f);
+                for (int i = 0; i < 8; i++) w[i] = kvs_two<FMT>(vn[i][g], e2, FMT == 0 ? 1.0f : scale_of(vsn[i][g]));
                 bool odd = false;
                 if (look) {
 #pragma unroll
@@ -303,94 +305,4 @@ template <int FMT> static int kvs_dim(const KvAttnArgs& a, int dim, int half, hi
         case 256: return kvs_launch<256, FMT>(a, half, st);
     }
     return 1;
-}
-int kr_launch_kv_step(const KvAttnArgs& a, int dim, int fmt, int half, hipStream_t st) {
-    return fmt == 0 ? kvs_dim<0>(a, dim, half, st) : fmt == 1 ? kvs_dim<1>(a, dim, half, st) : kvs_dim<2>(a, dim, half, st);
-}
-
-// Shares of split sequences joined.  FEW (eight shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares.  Else a unit is
-// one row: its threads divide the shares among themselves and meet in LDS.
-template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
-    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, FEW ? bm / 16 : bm);
-    if (it.b < 0) return;
-    const int rows = it.cnt * a.G, quads = dim / 4, tid = threadIdx.x, first = kv_item_of(a, it, bm, 0), step = a.kv_heads;      // a row tile's shares lie kv_heads items apart
-    const float* stats = a.ws + (size_t)a.items * bm * dim;
-    if constexpr (FEW) {
-        for (int i = tid; i < 16 * quads; i += 256) {
-            const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
-            if (rr >= rows) continue;
-            float ms[8], ls[8]; float4 x[8];
-            float top = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < 8; s++) {
-                const size_t at = (size_t)(first + min(s, it.nsplit - 1) * step) * bm + r;
-                ms[s] = stats[at * 2]; ls[s] = stats[at * 2 + 1]; x[s] = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
-                top = fmaxf(top, ms[s]);
-            }
-            const float base = top == -INFINITY ? 0.0f : top;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 8; s++) {
-                if (s >= it.nsplit || (ms[s] == -INFINITY && ls[s] == 0.0f)) continue;      // a share without keys of this row
-                const float f = __builtin_amdgcn_exp2f(ms[s] - base);
-                o.x += x[s].x * f; o.y += x[s].y * f; o.z += x[s].z * f; o.w += x[s].w * f;
-                den += ls[s] * f;
-            }
-            const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-            const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
-            *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
-        }
-    } else {
-        __shared__ float wl[KV_MAX_SHARES]; __shared__ float red[8]; __shared__ float4 sums[256];
-        const int r = it.split, rr = it.rt * bm + r;
-        if (rr >= rows) return;
-        float top = -INFINITY, den = 0.0f;
-        for (int s = tid; s < it.nsplit; s += 256) { const float ms = stats[((size_t)(first + s * step) * bm + r) * 2]; wl[s] = ms; top = fmaxf(top, ms); }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        if ((tid & 63) == 0) red[tid >> 6] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float base = top == -INFINITY ? 0.0f : top;
-        for (int s = tid; s < it.nsplit; s += 256) {
-            const float ms = wl[s], ls = stats[((size_t)(first + s * step) * bm + r) * 2 + 1];
-            const bool none = ms == -INFINITY && ls == 0.0f;
-            const float f = none ? -1.0f : __builtin_amdgcn_exp2f(ms - base);      // -1: a share without keys of this row
-            wl[s] = f;
-            if (!none) den += ls * f;
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) den += __shfl_xor(den, d);
-        if ((tid & 63) == 0) red[4 + (tid >> 6)] = den;
-        __syncthreads();
-        den = red[4] + red[5] + red[6] + red[7];
-        const int groups = 256 / quads, g = tid / quads, d = tid % quads * 4;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (g < groups) {
-            const float* wp = a.ws + ((size_t)first * bm + r) * dim + d;
-#pragma unroll 4
-            for (int s = g; s < it.nsplit; s += groups) {
-                const float f = wl[s];
-                const float4 x = *reinterpret_cast<const float4*>(wp + (size_t)s * step * bm * dim);
-                if (f != -1.0f) { o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f; }
-            }
-        }
-        sums[tid] = o;
-        __syncthreads();
-        if (tid >= quads) return;
-        for (int k = 1; k < groups; k++) { const float4 x = sums[k * quads + tid]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
-        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-        const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
-        *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
-    }
-}
-int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st) {
-    if (few) {
-        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-        else hipLaunchKernelGGL((kr_kv_join_kernel<false, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-    } else {
-        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-        else hipLaunchKernelGGL((kr_kv_join_kernel<false, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-    }
-    return 0;
 }

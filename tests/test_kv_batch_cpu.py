@@ -101,13 +101,13 @@ def c_call(**over):
     """kr_kv_attend on pointers that are never followed"""
     from krasis_amd import _lib
     lib = _lib.load_library()
-    cache = make_cache(2, over.pop("dim", 64), "mx8", 16, device="cpu")
-    a, b = states(cache, [20, 70])
+    cache = make_cache(2, over.pop("dim", 64), "mx8", 1024, device="cpu")
+    a, b = states(cache, [20, 16000])
     from krasis_amd.kv_cache import plan_of
     new = over.pop("new", 1)
     b.ensure_capacity(new)
     plan = plan_of(cache, [a, b], [1, new])
-    pages = _lib.KvPagesC(4096, 4096, 4096, 4096, 3, 16, 16, 2, cache.gqa_head_dim)
+    pages = _lib.KvPagesC(4096, 4096, 4096, 4096, 3, 16, 1024, 2, cache.gqa_head_dim)
     for k in ("format", "page_tokens", "n_pages", "kv_heads", "k", "k_scale"):
         if k in over:
             setattr(pages, k, over.pop(k))
@@ -122,7 +122,7 @@ def c_call(**over):
     (dict(page_tokens=32), "the plan is for"), (dict(n_pages=17), "the plan is for"), (dict(kv_heads=0), "heads"), (dict(dim=32), "heads of 32 channels"), (dict(heads=3), "do not divide"),
     (dict(heads=0), "do not divide"), (dict(window=-1), "window"), (dict(first=-2), "keep_first"), (dict(dtype=2), "bf16 or f16"), (dict(scale=float("nan")), "scale"), (dict(q=4104), "aligned"),
     (dict(out=None), "aligned"), (dict(qt=100), "multiples of 8"), (dict(parents=4096, new=65), "65 drafts"),
-    (dict(heads=32, new=70), "a workspace of 0 bytes")])
+    (dict(heads=32), "a workspace of 0 bytes")])
 def test_attention_refuses(over, text):
     with pytest.raises(ValueError, match=text):
         c_call(**dict(over))
@@ -168,7 +168,7 @@ def test_workspaces_grow_with_the_shares():
 
     def need(st, cnt, heads, window=0, tree=0):
         plan = plan_of(cache, st, cnt)
-        _lib.check(_lib.load_library().kr_kv_attend_workspace(ctypes.byref(pages), plan.data_ptr(), heads, window, 4, tree, ctypes.byref(size)))
+        _lib.check(_lib.load_library().kr_kv_attend_workspace(ctypes.byref(pages), plan.data_ptr(), heads, 0, window, 4, tree, ctypes.byref(size)))
         return size.value
     assert need([short], [1], 16) == 0 and need([long], [1], 16) > 0 and need([long], [40], 16, tree=1) > 0
     assert need([long], [1], 16, window=32) == 0
