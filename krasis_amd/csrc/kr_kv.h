@@ -44,20 +44,19 @@ struct KvAttnArgs {
 int kr_launch_kv_write(const KvRowsArgs& a, hipStream_t st);
 int kr_launch_kv_read(const KvRowsArgs& a, hipStream_t st);
 int kr_launch_kv_move(const KvMoveArgs& a, hipStream_t st);
-// by the width of the pages' numbers; half: q and out are f16; blocks: of 32 rows a wave
+// by the width of the pages' numbers; half: q and out are f16
 int kr_launch_kv_step_16(const KvAttnArgs& a, int dim, int half, hipStream_t st);
 int kr_launch_kv_step_8(const KvAttnArgs& a, int dim, int half, hipStream_t st);
 int kr_launch_kv_step_4(const KvAttnArgs& a, int dim, int half, hipStream_t st);
-int kr_launch_kv_tile_16(const KvAttnArgs& a, int dim, int half, int blocks, hipStream_t st);
-int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, int blocks, hipStream_t st);
-int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, int blocks, hipStream_t st);
+int kr_launch_kv_tile_16(const KvAttnArgs& a, int dim, int half, hipStream_t st);
+int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, hipStream_t st);
+int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, hipStream_t st);
 int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st);
 constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 
 constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step_dev.h
-constexpr int KV_TILE_KT = 64;       // keys of a tile in kr_kv_tile_dev.h, whose workgroups take 128 rows a block
-__host__ __device__ constexpr bool kv_tile_two(int dim, int fmt, int half) { return dim <= 128 && (!half || fmt == 0); }      // two blocks of 32 rows fit a wave's registers
-__host__ __device__ constexpr int kv_tile_waves(int dim, int blocks) { return dim <= 128 && blocks == 1 ? 2 : 1; }           // waves a SIMD holds
+constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile_dev.h
+__host__ __device__ constexpr int kv_tile_waves(int dim) { return dim <= 128 ? 2 : 1; }      // that a SIMD holds of the latter, by registers and LDS
 __host__ __device__ constexpr int kv_step_waves(int dim, int fmt) { return dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8; }      // of a workgroup in kr_kv_step_dev.h, one a CU: by registers
 constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
 

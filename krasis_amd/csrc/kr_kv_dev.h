@@ -39,6 +39,11 @@ template <bool H> __device__ __forceinline__ uint32_t kv_pack(float a, float b) 
 __device__ __forceinline__ kv_h2 kv_halves(uint32_t w) { return __builtin_bit_cast(kv_h2, w); }      // by value: a bit cast of a vector's element takes the vector's first
 __device__ __forceinline__ float kv_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float kv_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+// the sum of a packed pair and c, in 32 bits
+template <bool H> __device__ __forceinline__ float kv_sum2(uint32_t w, float c) {
+    if constexpr (H) return __builtin_amdgcn_fdot2(__builtin_bit_cast(kv_h2, w), __builtin_bit_cast(kv_h2, 0x3C003C00u), c, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(kv_b2, w), __builtin_bit_cast(kv_b2, 0x3F803F80u), c, false);
+}
 // what a packed pair of bf16 leaves of two floats
 __device__ __forceinline__ uint32_t kv_rest(float a, float b, uint32_t w) { return kv_pack<false>(a - kv_lo(w), b - kv_hi(w)); }
 
