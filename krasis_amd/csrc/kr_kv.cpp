@@ -41,8 +41,7 @@ int check_pages(const kr_kv_pages* p, const int* plan, KvPages& o) {
     if ((int64_t)p->page_tokens * p->n_pages * (o.row_bytes / 16) > UINT32_MAX) return kr_fail(KR_ERR_VALUE, "kr_kv: %d pages of %d tokens are more than 64 GiB", p->n_pages, p->page_tokens);
     o.row16 = (uint32_t)o.row_bytes / 16; o.scale_and = scaled(p->format) ? 0xFFu : 0u; o.scale_or = scaled(p->format) ? 0u : 127u;
     o.scale_shift = p->format == KR_KV_MX8 ? 1 : 0;
-    o.page_tokens = p->page_tokens;
-    o.page_magic = p->page_tokens == 1 ? 0xFFFFFFFFu : (uint32_t)((1ull << 32) / (uint64_t)p->page_tokens);
+    o.page = kv_divisor((uint32_t)p->page_tokens);
     return KR_OK;
 }
 KvSeqs seqs_of(const int* plan, const int* dev) {
@@ -87,7 +86,7 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
     for (int b = 0; b < h.batch; b++) {
         const int cnt = h.row0[b + 1] - h.row0[b]; const int64_t rows = (int64_t)cnt * G;
         if (rows < p.min_rows || rows > p.max_rows) continue;
-        const int n = kv_tiles_ub(h.lens[b], cnt, G, window, first, tree, p.bm, p.kt);
+        const int n = kv_tiles_ub(h.lens[b], cnt, kv_divisor((uint32_t)G), window, first, tree, p.bm, p.kt);
         const int64_t rt = (int64_t)kv_row_tiles(cnt, G, p.bm) * kv_heads;
         if (cnt > 1) p.one = false;
         seqs.push_back({n, rt}); total += rt * n; whole += rt; longest = n > longest ? n : longest;
@@ -114,7 +113,7 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
         most = ns > most ? ns : most;
     }
     p.shares = most;
-    p.few = most <= 8;
+    p.few = most <= 16;
     if (p.split) for (const Seq& s : seqs) if (s.tiles > p.tps) p.units += s.row_tiles * (p.few ? p.bm / 16 : p.bm);
 }
 void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, int window, int first, bool tree, Part* p) {
@@ -220,7 +219,7 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
     if (q_token_stride % 8 || q_head_stride % 8) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: strides must be multiples of 8 elements");
     a.s = seqs_of(plan, dev_plan);
     a.q = (const uint16_t*)q; a.out = (uint16_t*)out; a.q_tok = q_token_stride; a.q_head = q_head_stride; a.parents = parents;
-    a.heads = heads; a.kv_heads = p->kv_heads; a.G = heads / p->kv_heads;
+    a.heads = heads; a.kv_heads = kv_divisor((uint32_t)p->kv_heads); a.G = kv_divisor((uint32_t)(heads / p->kv_heads));
     a.window = window; a.first = clamp_first(h, window, keep_first);
     a.scale_log2 = scale * 1.44269504088896340736f;
     Part part[2];
@@ -234,7 +233,7 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
     static int (*const tile[3])(const KvAttnArgs&, int, int, hipStream_t) = {kr_launch_kv_tile_16, kr_launch_kv_tile_8, kr_launch_kv_tile_4};
     for (int i = 1; i >= 0; i--) {                            // prompts first, they take longest
         if (!part[i].items) continue;
-        a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = part[i].tps; a.items = (int)part[i].items; a.one = part[i].one;
+        a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = kv_divisor((uint32_t)part[i].tps); a.items = (int)part[i].items; a.one = part[i].one;
         a.ws = (float*)((char*)workspace + (i ? b0 : 0));
         if (int rc = launched("kr_kv_attend", i ? tile[fmt](a, p->dim, half, st) : step[fmt](a, p->dim, half, st))) return rc;
         if (part[i].split)

@@ -6,6 +6,9 @@
 
 #include "../../include/krasis_hip.h"
 
+struct KvDiv { uint32_t d, magic; };      // a divisor and floor(2^32 / d), at most 2^32 - 1
+inline KvDiv kv_divisor(uint32_t d) { return KvDiv{d, d == 1 ? 0xFFFFFFFFu : (uint32_t)((1ull << 32) / d)}; }
+
 // one layer's pages: keys / values [slots][kv_heads][dim] in the page format, scales [slots][kv_heads][dim / 32] for the microscaled ones; slot = page * page_tokens + offset
 struct KvPages {
     uint8_t *k, *v, *ks, *vs;
@@ -14,8 +17,7 @@ struct KvPages {
     uint32_t row16;                    // row_bytes / 16: places in the pages are counted in units of 16 bytes
     uint32_t scale_and, scale_or;      // (scale byte & scale_and) | scale_or: pages of plain E4M3 give any byte of theirs, which becomes 127
     int scale_shift;                   // place in the pages >> scale_shift = place of its scales
-    int page_tokens;
-    uint32_t page_magic;               // floor(2^32 / page_tokens), at most 2^32 - 1: kv_page() below
+    KvDiv page;                        // tokens
 };
 // the sequences of a step, on the device
 struct KvSeqs {
@@ -32,11 +34,12 @@ struct KvAttnArgs {
     const uint16_t* q; uint16_t* out;
     long q_tok, q_head;                // strides in elements; out is [rows][heads][dim]
     const int* parents;                // drafted trees: parent draft of every new row, or NULL
-    int heads, kv_heads, G;            // G = heads / kv_heads
+    int heads;
+    KvDiv kv_heads, G;                 // G = heads / kv_heads
     int window, first;
     float scale_log2;                  // scale * log2(e): scores are kept in units of log 2
     int min_rows, max_rows;            // the sequences of this launch: those whose new rows times G lie in between
-    int tps;                           // key tiles a workgroup takes at most
+    KvDiv tps;                         // key tiles a workgroup takes at most
     int items, one;                    // one: no sequence of this launch has more than one new token, and there are no trees
     float* ws;                         // partial results of sequences that are split: [item][KV_BM rows][dim] sums, then [item][rows][2] maximum and denominator
 };
@@ -62,10 +65,10 @@ constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: 
 
 // ---- the division of a launch into items, the same on the host (how many) and on the device (which one)
 // key tiles that any row tile of a sequence can need; BM rows and KT keys a tile
-__host__ __device__ inline int kv_tiles_ub(int len, int cnt, int G, int window, int first, bool tree, int bm, int kt) {
+__host__ __device__ inline int kv_tiles_ub(int len, int cnt, KvDiv G, int window, int first, bool tree, int bm, int kt) {
     const int all = (len + kt - 1) / kt;
     if (window <= 0) return all;
-    const long span = (long)window + (tree ? cnt : (bm - 1) / G + 1);      // tokens from the first row's window to the last row
+    const long span = (long)window + (tree ? cnt : (int)(((uint64_t)(bm - 1) * G.magic) >> 32) + 2);      // tokens from the first row's window to the last row, or one more
     const int some = (int)((span < len ? span : len) / kt) + 2 + (first + kt - 1) / kt;
     return some < all ? some : all;
 }

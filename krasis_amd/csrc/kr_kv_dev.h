@@ -10,17 +10,19 @@ typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
 typedef float kv_f4 __attribute__((ext_vector_type(4)));
 typedef float kv_f16 __attribute__((ext_vector_type(16)));
 
-// j / page_tokens for 0 <= j < 2^31: the high product is short by at most one
-__device__ __forceinline__ uint32_t kv_page(const KvPages& p, uint32_t j, uint32_t& off) {
-    uint32_t n = __umulhi(j, p.page_magic);
-    off = j - n * (uint32_t)p.page_tokens;
-    if (off >= (uint32_t)p.page_tokens) { n++; off -= (uint32_t)p.page_tokens; }
+// x / d for 0 <= x < 2^32 with the d's floor(2^32 / d), at most 2^32 - 1: the high product is short by at most one
+__host__ __device__ __forceinline__ uint32_t kv_div(uint32_t x, KvDiv d, uint32_t& rest) {
+    uint32_t n = (uint32_t)(((uint64_t)x * d.magic) >> 32);
+    rest = x - n * d.d;
+    if (rest >= d.d) { n++; rest -= d.d; }
     return n;
 }
+__host__ __device__ __forceinline__ uint32_t kv_div(uint32_t x, KvDiv d) { uint32_t rest; return kv_div(x, d, rest); }
+__device__ __forceinline__ uint32_t kv_page(const KvPages& p, uint32_t j, uint32_t& off) { return kv_div(j, p.page, off); }
 __device__ __forceinline__ uint32_t kv_slot(const KvPages& p, const int* table, uint32_t j) {
     uint32_t off;
     const uint32_t n = kv_page(p, j, off);
-    return (uint32_t)table[n] * (uint32_t)p.page_tokens + off;
+    return (uint32_t)table[n] * p.page.d + off;
 }
 
 // two neighbouring codes of a dword times the scale as a packed pair of bf16.  E4M3 and E2M1 have at most four significant bits and scales are powers of two of at least 2^-100:
@@ -63,44 +65,51 @@ __device__ __forceinline__ uint64_t kv_ancestors(const int* parents, int n, int 
     return seen;
 }
 
-struct KvItem { int b, rt, split, kvh, nsplit, len, cnt, row0, page0, base; };      // base: the sequence's first item
+// inclusive sum over the lanes
+__device__ __forceinline__ int kv_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);      // one, two, four, eight lanes up within rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);     // row 0's sum to row 1, row 2's to row 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);     // the first half's to the second
+    return x;
+}
+
+struct KvItem { int b, rt, split, kvh, nsplit, len, cnt, row0, page0, base, row_tiles; };      // base: the sequence's first item
 // item -> sequence, row tile, share of the keys, head.  A lane counts the items of one sequence, 64 sequences at a time; heads lie side by side (they read the same lines of scales),
-// the last row tiles first (a prompt's last rows see the most keys).  sub: parts of a row tile in a launch over row tiles alone (shares = 1).
-template <bool SHARES> __device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, int idx, int bm, int kt, int sub) {
+// the last row tiles first (a prompt's last rows see the most keys).  In a launch over row tiles alone (SHARES false) each has `sub` parts.
+template <bool SHARES> __device__ __forceinline__ KvItem kv_item(const KvAttnArgs& a, int idx, int bm, int kt, KvDiv sub) {
     const int lane = threadIdx.x & 63;
     KvItem it;
     int base = 0, ibase = 0;
     for (int b0 = 0; b0 < a.s.batch; b0 += 64) {
         const int b = b0 + lane;
-        int n = 0, full = 0, len = 0, cnt = 0, ns = 1, row0 = 0, page0 = 0;
+        int n = 0, full = 0, len = 0, cnt = 0, ns = 1, row0 = 0, page0 = 0, rts = 0;
         if (b < a.s.batch) {
             row0 = a.s.row0[b]; cnt = a.s.row0[b + 1] - row0; len = a.s.lens[b]; page0 = a.s.page0[b];
-            const int rows = cnt * a.G;
+            const int rows = cnt * (int)a.G.d;
             if (rows >= a.min_rows && rows <= a.max_rows) {
-                ns = (kv_tiles_ub(len, cnt, a.G, a.window, a.first, a.parents != nullptr, bm, kt) + a.tps - 1) / a.tps;
-                const int rts = kv_row_tiles(cnt, a.G, bm);
-                full = rts * ns * a.kv_heads;
-                n = SHARES ? full : (ns > 1 ? rts * sub * a.kv_heads : 0);
+                ns = (int)kv_div((uint32_t)(kv_tiles_ub(len, cnt, a.G, a.window, a.first, a.parents != nullptr, bm, kt) + (int)a.tps.d - 1), a.tps);
+                rts = kv_row_tiles(cnt, (int)a.G.d, bm);
+                full = rts * ns * (int)a.kv_heads.d;
+                n = SHARES ? full : (ns > 1 ? rts * (int)(sub.d * a.kv_heads.d) : 0);
             }
         }
-        int end = n, iend = full;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(end, d), y = SHARES ? 0 : __shfl_up(iend, d);
-            if (lane >= d) { end += x; iend += y; }
-        }
+        const int end = kv_scan(n), iend = SHARES ? 0 : kv_scan(full);
         const uint64_t hit = __ballot(base + end > idx);
         if (hit) {
             const int w = __builtin_ctzll(hit);
             it.b = b0 + w;
             it.nsplit = __builtin_amdgcn_readlane(ns, w); it.len = __builtin_amdgcn_readlane(len, w); it.cnt = __builtin_amdgcn_readlane(cnt, w); it.row0 = __builtin_amdgcn_readlane(row0, w);
+            it.page0 = __builtin_amdgcn_readlane(page0, w); it.row_tiles = __builtin_amdgcn_readlane(rts, w);
             const int e = __builtin_amdgcn_readlane(end, w), nn = __builtin_amdgcn_readlane(n, w);
-            int r = idx - (base + e - nn);
             it.base = SHARES ? base + e - nn : ibase + __builtin_amdgcn_readlane(iend, w) - __builtin_amdgcn_readlane(full, w);
-            it.kvh = r % a.kv_heads; r /= a.kv_heads;
-            const int per = SHARES ? it.nsplit : sub;
-            it.split = r % per; it.rt = kv_row_tiles(it.cnt, a.G, bm) - 1 - r / per;
-            it.page0 = __builtin_amdgcn_readlane(page0, w);
+            uint32_t kvh;
+            const uint32_t r = kv_div((uint32_t)(idx - (base + e - nn)), a.kv_heads, kvh);
+            it.kvh = (int)kvh;
+            if (SHARES) { const uint32_t t = it.nsplit == 1 ? r : r / (uint32_t)it.nsplit; it.split = (int)(r - t * it.nsplit); it.rt = it.row_tiles - 1 - (int)t; }
+            else { uint32_t part; it.rt = it.row_tiles - 1 - (int)kv_div(r, sub, part); it.split = (int)part; }
             return it;
         }
         base += __builtin_amdgcn_readlane(end, 63);
@@ -110,8 +119,8 @@ template <bool SHARES> __device__ __forceinline__ KvItem kv_item(const KvAttnArg
     return it;
 }
 // the item that holds a row tile's share, for the one who joins them
-__device__ __forceinline__ int kv_item_of(const KvAttnArgs& a, const KvItem& it, int bm, int split) {
-    return it.base + ((kv_row_tiles(it.cnt, a.G, bm) - 1 - it.rt) * it.nsplit + split) * a.kv_heads + it.kvh;
+__device__ __forceinline__ int kv_item_of(const KvAttnArgs& a, const KvItem& it, int split) {
+    return it.base + ((it.row_tiles - 1 - it.rt) * it.nsplit + split) * (int)a.kv_heads.d + it.kvh;
 }
 
 // the keys of a row tile: tiles of kept first keys that lie apart from the window's, then one range
@@ -119,8 +128,8 @@ struct KvRange { int lo, hi, kept, start, tiles, before, t0, t1; };      // [lo,
 __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& it, int bm, int kt) {
     KvRange r;
     r.before = it.len - it.cnt;
-    r.t0 = it.rt * bm / a.G;
-    r.t1 = min(it.cnt, ((it.rt + 1) * bm - 1) / a.G + 1);
+    r.t0 = (int)kv_div((uint32_t)(it.rt * bm), a.G);
+    r.t1 = min(it.cnt, (int)kv_div((uint32_t)((it.rt + 1) * bm - 1), a.G) + 1);
     r.hi = r.before + r.t1;                  // a draft's ancestors come before it
     r.lo = 0; r.kept = 0; r.start = 0;
     if (a.window > 0) {

@@ -1,36 +1,40 @@
 // kr_kv_join.hip -- the second launch of attention over the paged cache, where sequences were shared out among workgroups.
 #include "kr_kv_dev.h"
 
-// Shares of split sequences joined.  FEW (eight shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares.  Else a unit is
+// Shares of split sequences joined.  FEW (16 shares at most): a unit is 16 rows of a row tile and one head, a thread holds four columns of a row and walks the shares, four at a time.  Else a unit is
 // one row: its threads divide the shares among themselves and meet in LDS.
-template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt) {
-    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, FEW ? bm / 16 : bm);
+template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_kernel(const KvAttnArgs a, int dim, int bm, int kt, KvDiv sub) {
+    const KvItem it = kv_item<false>(a, blockIdx.x, bm, kt, sub);
     if (it.b < 0) return;
-    const int rows = it.cnt * a.G, quads = dim / 4, tid = threadIdx.x, first = kv_item_of(a, it, bm, 0), step = a.kv_heads;      // a row tile's shares lie kv_heads items apart
+    const int G = (int)a.G.d, rows = it.cnt * G, quads = dim / 4, tid = threadIdx.x, first = kv_item_of(a, it, 0), step = (int)a.kv_heads.d;      // a row tile's shares lie kv_heads items apart
     const float* stats = a.ws + (size_t)a.items * bm * dim;
     if constexpr (FEW) {
         for (int i = tid; i < 16 * quads; i += 256) {
             const int r = it.split * 16 + i / quads, d = i % quads * 4, rr = it.rt * bm + r;
             if (rr >= rows) continue;
-            float ms[8], ls[8]; float4 x[8];
-            float top = -INFINITY;
+            float top = -INFINITY, den = 0.0f; float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float* sp = stats + ((size_t)first * bm + r) * 2; const float* wp = a.ws + ((size_t)first * bm + r) * dim + d;
+            const size_t next = (size_t)step * bm;
+            for (int s0 = 0; s0 < it.nsplit; s0 += 4) {       // four shares at a time, measured from the largest maximum so far
+                float ms[4], ls[4]; float4 x[4];
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                const size_t at = (size_t)(first + min(s, it.nsplit - 1) * step) * bm + r;
-                ms[s] = stats[at * 2]; ls[s] = stats[at * 2 + 1]; x[s] = *reinterpret_cast<const float4*>(a.ws + at * dim + d);
-                top = fmaxf(top, ms[s]);
-            }
-            const float base = top == -INFINITY ? 0.0f : top;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f); float den = 0.0f;
+                for (int u = 0; u < 4; u++) {
+                    const size_t s = (size_t)min(s0 + u, it.nsplit - 1) * next;
+                    ms[u] = sp[s * 2]; ls[u] = sp[s * 2 + 1]; x[u] = *reinterpret_cast<const float4*>(wp + s * dim);
+                }
+                const float mx = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), top), base = mx == -INFINITY ? 0.0f : mx, was = __builtin_amdgcn_exp2f(top - base);
+                if (s0) { o.x *= was; o.y *= was; o.z *= was; o.w *= was; den *= was; }
+                top = mx;
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                if (s >= it.nsplit || (ms[s] == -INFINITY && ls[s] == 0.0f)) continue;      // a share without keys of this row
-                const float f = __builtin_amdgcn_exp2f(ms[s] - base);
-                o.x += x[s].x * f; o.y += x[s].y * f; o.z += x[s].z * f; o.w += x[s].w * f;
-                den += ls[s] * f;
+                for (int u = 0; u < 4; u++) {
+                    if (s0 + u >= it.nsplit || (ms[u] == -INFINITY && ls[u] == 0.0f)) continue;      // a share without keys of this row
+                    const float f = __builtin_amdgcn_exp2f(ms[u] - base);
+                    o.x += x[u].x * f; o.y += x[u].y * f; o.z += x[u].z * f; o.w += x[u].w * f;
+                    den += ls[u] * f;
+                }
             }
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-            const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
+            const int t = (int)kv_div((uint32_t)rr, a.G), h = it.kvh * G + rr - t * G;
             *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
         }
     } else {
@@ -73,17 +77,18 @@ template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_ke
         if (tid >= quads) return;
         for (int k = 1; k < groups; k++) { const float4 x = sums[k * quads + tid]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-        const int t = rr / a.G, h = it.kvh * a.G + rr - t * a.G;
+        const int t = (int)kv_div((uint32_t)rr, a.G), h = it.kvh * G + rr - t * G;
         *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
     }
 }
 int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st) {
+    const KvDiv sub = kv_divisor((uint32_t)(few ? bm / 16 : bm));
     if (few) {
-        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-        else hipLaunchKernelGGL((kr_kv_join_kernel<false, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt, sub);
+        else hipLaunchKernelGGL((kr_kv_join_kernel<false, true>), dim3(units), dim3(256), 0, st, a, dim, bm, kt, sub);
     } else {
-        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
-        else hipLaunchKernelGGL((kr_kv_join_kernel<false, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt);
+        if (half) hipLaunchKernelGGL((kr_kv_join_kernel<true, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt, sub);
+        else hipLaunchKernelGGL((kr_kv_join_kernel<false, false>), dim3(units), dim3(256), 0, st, a, dim, bm, kt, sub);
     }
     return 0;
 }

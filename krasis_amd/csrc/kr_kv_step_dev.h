@@ -47,12 +47,12 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     constexpr int C = KvsCols<DIM>::C, GROUPS = KvsCols<DIM>::GROUPS, VB = C * BITS / 8, VW = VB < 4 ? 1 : VB / 4;
     constexpr int NB = DIM == 64 || DIM == 128 ? 1 : 2;       // blocks of 32 channels that a quarter of a row meets
     extern __shared__ float kvs_lds_[];
-    const KvItem it = kv_item<true>(a, blockIdx.x, 16, KV_STEP_KT, 1);
+    const KvItem it = kv_item<true>(a, blockIdx.x, 16, KV_STEP_KT, KvDiv{});
     if (it.b < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, q = lane >> 4;
     const KvRange rg = kv_range(a, it, 16, KV_STEP_KT);
-    const int c0 = it.split * a.tps, c1 = min(rg.tiles, c0 + a.tps);
-    const int rows = it.cnt * a.G, r = min(row, rows - 1), t = r / a.G, head = it.kvh * a.G + r - t * a.G;
+    const int c0 = it.split * (int)a.tps.d, c1 = min(rg.tiles, c0 + (int)a.tps.d);
+    const int G = (int)a.G.d, rows = it.cnt * G, r = min(row, rows - 1), t = (int)kv_div((uint32_t)r, a.G), head = it.kvh * G + r - t * G;
     const int* table = a.s.pages + it.page0;
     const uint8_t* kbase = a.p.k + (size_t)it.kvh * a.p.head_bytes + q * KB;
     const uint8_t* vbase = a.p.v + (size_t)it.kvh * a.p.head_bytes;
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
         }
         if (whole) {
             const float inv = dt[rr] == 0.0f ? 0.0f : 1.0f / dt[rr];
-            const int tt = rr / a.G, hh = it.kvh * a.G + rr - tt * a.G;
+            const int tt = (int)kv_div((uint32_t)rr, a.G), hh = it.kvh * G + rr - tt * G;
             u32x2 o = {kv_pack<HQ>(s.x * inv, s.y * inv), kv_pack<HQ>(s.z * inv, s.w * inv)};
             *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + tt) * a.heads + hh) * DIM + d) = o;
         } else *reinterpret_cast<float4*>(wo + rr * DIM + d) = s;

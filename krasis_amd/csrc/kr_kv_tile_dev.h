@@ -35,13 +35,13 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     uint32_t* Sl = (uint32_t*)(Vs + 2 * KT * LDV);            // [NS][KT] where the keys of tile c lie, in units of 16 bytes, at c modulo NS
     int* Dp = (int*)(Sl + NS * KT);                           // [KV_MAX_TREE] depths of the drafts
     int* Odd = Dp + KV_MAX_TREE;                              // some value of a tile that not all rows see was not finite
-    const KvItem it = kv_item<true>(a, blockIdx.x, BM, KT, 1);
+    const KvItem it = kv_item<true>(a, blockIdx.x, BM, KT, KvDiv{});
     if (it.b < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
     const KvRange rg = kv_range(a, it, BM, KT);
-    const int c0 = it.split * a.tps, c1 = min(rg.tiles, c0 + a.tps);
-    const int rows = it.cnt * a.G, rw = it.rt * BM + wave * 32;
-    const int w0 = min(it.cnt - 1, rw / a.G), w1 = min(it.cnt - 1, (rw + 31) / a.G);      // the wave's first and last token
+    const int c0 = it.split * (int)a.tps.d, c1 = min(rg.tiles, c0 + (int)a.tps.d);
+    const int G = (int)a.G.d, rows = it.cnt * G, rw = it.rt * BM + wave * 32;
+    const int w0 = min(it.cnt - 1, (int)kv_div((uint32_t)rw, a.G)), w1 = min(it.cnt - 1, (int)kv_div((uint32_t)(rw + 31), a.G));      // the wave's first and last token
     const int* table = a.s.pages + it.page0;
     const float scale = fmaxf(fabsf(a.scale_log2), 1.1754944e-38f);      // its sign goes into the queries: scores that are not seen are -infinity before it, too
 
@@ -54,12 +54,12 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     u32x4 qf[NP][KS];
     {
         const int r = min(rw + col, rows - 1);
-        tk = r / a.G; pos = rg.before + tk; seen = 0;
+        tk = (int)kv_div((uint32_t)r, a.G); pos = rg.before + tk; seen = 0;
         if (a.parents) {
             seen = (uint64_t)__shfl((uint32_t)(all >> 32), tk) << 32 | __shfl((uint32_t)all, tk);
             pos = rg.before + __popcll(seen) - 1;
         }
-        const uint16_t* qp = a.q + (size_t)(it.row0 + tk) * a.q_tok + (size_t)(it.kvh * a.G + r - tk * a.G) * a.q_head + 8 * h;
+        const uint16_t* qp = a.q + (size_t)(it.row0 + tk) * a.q_tok + (size_t)(it.kvh * G + r - tk * G) * a.q_head + 8 * h;
         const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     auto place = [&](int c, int k) {
         uint32_t in;
         const uint32_t n = page_of(c, k, in);
-        return ((uint32_t)table[n] * (uint32_t)a.p.page_tokens + in) * a.p.row16;
+        return ((uint32_t)table[n] * a.p.page.d + in) * a.p.row16;
     };
     // this thread's chunks: row of the tile, place in the row
     u32x4 kn[PT], vn[PT]; uint32_t ksn[PT], vsn[PT], off[PT], coming[PT];
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
             settle(sb);
             places(c + 3, coming);
             sums(c, 1, c + 1, 1, yes());
-            if (turn == 1) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page * (uint32_t)a.p.page_tokens + in) * a.p.row16;
+            if (turn == 1) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page * a.p.page.d + in) * a.p.row16;
         }
         __syncthreads();
         if (*Odd) {                                           // the values that became 0 above: every row takes those that it sees
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
         if (r >= rows) return;
         if (it.nsplit == 1) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint16_t* op = a.out + ((size_t)(it.row0 + tk) * a.heads + it.kvh * a.G + r - tk * a.G) * DIM + 4 * h;
+            uint16_t* op = a.out + ((size_t)(it.row0 + tk) * a.heads + it.kvh * G + r - tk * G) * DIM + 4 * h;
 #pragma unroll
             for (int d = 0; d < DB; d++)
 #pragma unroll

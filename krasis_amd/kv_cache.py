@@ -25,6 +25,7 @@ _ROWS = {torch.bfloat16: 0, torch.float16: 1}            # KR_KV_*
 _PAGES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 _MICROSCALED = {"mx8": 3, "mx4": 4}
 MAX_DRAFTS = 64                  # of one sequence in a tree
+_Strides = ctypes.c_int64 * 4
 
 
 class PagedKVCache:
@@ -278,50 +279,55 @@ class KVBatch:
             if not 0 <= layer < c.num_layers:
                 raise ValueError(f"layer {layer} of {c.num_layers}")
             at = lambda t: None if t is None else t[layer].data_ptr()
-            self._pages[layer] = p = _lib.KvPagesC(at(c.k_cache), at(c.v_cache), at(c.k_scale), at(c.v_scale), self._format, c.page_size, c.max_pages, c.num_kv_heads, c.gqa_head_dim)
-        return ctypes.byref(p)
+            p = _lib.KvPagesC(at(c.k_cache), at(c.v_cache), at(c.k_scale), at(c.v_scale), self._format, c.page_size, c.max_pages, c.num_kv_heads, c.gqa_head_dim)
+            self._pages[layer] = p = ctypes.byref(p)
+        return p
 
     def _call(self, fn, *args) -> None:
-        stream = torch.cuda.current_stream(self.device)
-        if stream.cuda_stream != self._stream:
-            self._dev.record_stream(stream)              # the plan's memory is not given to anyone else before this stream is done with it
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(*args, stream.cuda_stream or 1)
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)      # torch.cuda.current_stream() without the objects around it: steps are made of calls of a few microseconds
+        if stream != self._stream:
+            self._dev.record_stream(torch.cuda.current_stream(self.device))      # the plan's memory is not given to anyone else before this stream is done with it
+        if torch._C._cuda_getDevice() == self.device.index:
+            rc = fn(*args, stream or 1)
         else:
             with torch.cuda.device(self.device):
-                rc = fn(*args, stream.cuda_stream or 1)
+                rc = fn(*args, stream or 1)
         if rc:
             _lib.check(rc)
 
-    def _rows_of(self, name: str, t: torch.Tensor, heads: int, exact_heads: bool = True) -> torch.Tensor:
-        d = self.cache.gqa_head_dim
+    def _rows_of(self, name: str, t: torch.Tensor, heads: int):
+        """the rows as a kernel takes them, the two strides and the number of heads; heads 0: any number"""
+        d, shape = self.cache.gqa_head_dim, t.shape
         if t.device != self.device or t.dtype not in _ROWS:
             raise ValueError(f"{name}: bfloat16 or float16 rows on {self.device}, not {t.dtype} on {t.device}")
-        if t.dim() == 2 and t.shape[1] % d == 0:
-            t = t.unflatten(1, (t.shape[1] // d, d))
-        if t.dim() != 3 or t.shape[0] != self.rows or t.shape[2] != d or (exact_heads and t.shape[1] != heads):
-            raise ValueError(f"{name}: {tuple(t.shape)} for {self.rows} rows of {heads if exact_heads else 'any'} heads of {d} channels")
-        if (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16) and t.numel():
+        if len(shape) == 2 and shape[1] % d == 0:
+            t = t.unflatten(1, (shape[1] // d, d))
+            shape = t.shape
+        if len(shape) != 3 or shape[0] != self.rows or shape[2] != d or (heads and shape[1] != heads):
+            raise ValueError(f"{name}: {tuple(shape)} for {self.rows} rows of {heads or 'any'} heads of {d} channels")
+        st, sh, sd = t.stride()
+        if (sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16) and t.numel():
             t = t.clone(memory_format=torch.contiguous_format)
-        return t
+            st, sh, sd = t.stride()
+        return t, st, sh, shape[1]
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """The new tokens' keys and values `[rows, kv_heads, dim]` (or `[rows, kv_heads * dim]`) into the pages, in the pages' format."""
-        k, v = self._rows_of("k", k, self.cache.num_kv_heads), self._rows_of("v", v, self.cache.num_kv_heads)
+        h = self.cache.num_kv_heads
+        k, kt, kh, _ = self._rows_of("k", k, h)
+        v, vt, vh, _ = self._rows_of("v", v, h)
         if k.dtype != v.dtype:
             raise ValueError(f"k is {k.dtype}, v is {v.dtype}")
-        strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        self._call(self._lib.kr_kv_write, self._layer(layer), *self._plan, k.data_ptr(), v.data_ptr(), strides, _ROWS[k.dtype])
+        self._call(self._lib.kr_kv_write, self._layer(layer), *self._plan, k.data_ptr(), v.data_ptr(), _Strides(kt, kh, vt, vh), _ROWS[k.dtype])
 
     def read(self, layer: int, dtype: torch.dtype = torch.float16):
         """The new tokens' keys and values as the pages hold them, `[rows, kv_heads, dim]` each, rounded once to `dtype` (bfloat16 or float16)."""
         if dtype not in _ROWS:
             raise ValueError(f"rows are read as bfloat16 or float16, not {dtype}")
-        c = self.cache
-        k = torch.empty((self.rows, c.num_kv_heads, c.gqa_head_dim), dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
-        strides = (ctypes.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        self._call(self._lib.kr_kv_read, self._layer(layer), *self._plan, k.data_ptr(), v.data_ptr(), strides, _ROWS[dtype])
+        h, d = self.cache.num_kv_heads, self.cache.gqa_head_dim
+        k = torch.empty((self.rows, h, d), dtype=dtype, device=self.device)
+        v = torch.empty((self.rows, h, d), dtype=dtype, device=self.device)
+        self._call(self._lib.kr_kv_read, self._layer(layer), *self._plan, k.data_ptr(), v.data_ptr(), _Strides(h * d, d, h * d, d), _ROWS[dtype])
         return k, v
 
     def attend(self, layer: int, q: torch.Tensor, scale: Optional[float] = None, window: int = 0, keep_first: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -363,8 +369,8 @@ class KVBatch:
         return torch.tensor(parents, dtype=torch.int32, device=self.device)
 
     def _attend(self, layer, q, parents, scale, window, keep_first, out):
-        q = self._rows_of("q", q, 0, exact_heads=False)
-        heads, d = q.shape[1], q.shape[2]
+        q, qt, qh, heads = self._rows_of("q", q, 0)
+        d = self.cache.gqa_head_dim
         if out is None:
             out = torch.empty((self.rows, heads, d), dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
@@ -376,7 +382,7 @@ class KVBatch:
             _lib.check(self._lib.kr_kv_attend_workspace(pages, self._plan[0], heads, window, keep_first, int(parents is not None), ctypes.byref(size)))
             self._need[key] = need = size.value
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None      # of this call alone: two streams, or two graphs, never share one
-        self._call(self._lib.kr_kv_attend, pages, *self._plan, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), _ROWS[q.dtype], heads, d ** -0.5 if scale is None else scale,
+        self._call(self._lib.kr_kv_attend, pages, *self._plan, q.data_ptr(), qt, qh, out.data_ptr(), _ROWS[q.dtype], heads, d ** -0.5 if scale is None else scale,
                    window, keep_first, None if parents is None else parents.data_ptr(), None if ws is None else ws.data_ptr(), need)
         return out
 
