@@ -5,7 +5,8 @@
 //   S^T[key][row] = K Q^T    first operand: 16 key rows; a lane holds a quarter of a row, so a microscaled row costs it one scale and loads of 16 bytes
 //   O^T[d][row] += V^T P^T   a lane holds 8 keys and c neighbouring columns; byte permutes make them the columns' fragments
 // A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a running maximum and sum per row, and
-// meet in LDS.  Weights are taken as two bf16 pieces (16 bits), f16 queries over bf16-converted pages too: the matrix cores have time for it here.
+// meet in LDS.  Weights are rounded to the products' type, half a step of 2^-8 in bf16, as far as the result is rounded itself; f16 queries over pages that become bf16, and their weights, are
+// taken as two bf16 pieces (16 bits).
 #pragma once
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
@@ -42,7 +43,7 @@ template <int DIM, int FMT, bool HQ, bool ONE>
 __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DIM, FMT) / 4) kr_kv_step_kernel(const KvAttnArgs a) {
     constexpr int WAVES = kv_step_waves(DIM, FMT);
     constexpr bool HM = HQ && FMT == 0;                       // f16 products
-    constexpr int QP = HQ && !HM ? 2 : 1, PP = HM ? 1 : 2;    // pieces of a query and of a weight
+    constexpr int NP = HQ && !HM ? 2 : 1;                     // bf16 pieces of an f16 query and of its weights
     constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, U = DIM / 32, KB = DIM / 4 * BITS / 8, KW = KB / 4;
     constexpr int C = KvsCols<DIM>::C, GROUPS = KvsCols<DIM>::GROUPS, VB = C * BITS / 8, VW = VB < 4 ? 1 : VB / 4;
     constexpr int NB = DIM == 64 || DIM == 128 ? 1 : 2;       // blocks of 32 channels that a quarter of a row meets
@@ -68,13 +69,14 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
         pos = rg.before + __shfl(depth, t);
     }
     // the query row: dims q DIM / 4 + 8 i
-    u32x4 qf[QP][U];
+    u32x4 qf[NP][U];
     {
         const uint16_t* qp = a.q + (size_t)(it.row0 + t) * a.q_tok + (size_t)head * a.q_head + q * (DIM / 4);
+        const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 8 * i);
-            if constexpr (QP == 1) qf[0][i] = x;
+            const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 8 * i) ^ sign;
+            if constexpr (NP == 1) qf[0][i] = x;
             else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -121,7 +123,8 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
         }
     };
 
-    float m = -INFINITY, l = 0.0f;
+    const float scale = fmaxf(fabsf(a.scale_log2), 1.1754944e-38f);      // its sign goes into the queries: scores that are not seen are -infinity before it, too
+    float m = -INFINITY, l = 0.0f, base = 0.0f, most = -1.0f;
     kv_f4 acc[DIM / 16];
 #pragma unroll
     for (int j = 0; j < DIM / 16; j++) acc[j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -150,49 +153,64 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
 #pragma unroll
                 for (int e = 0; e < 4; e++) kf[e] = kvs_two<FMT>(&kn[b][i * KW / U], e, s);
 #pragma unroll
-                for (int p = QP - 1; p >= 0; p--) st[b] = kvs_mfma<HM>(kf, qf[p][i], st[b]);
+                for (int p = NP - 1; p >= 0; p--) st[b] = kvs_mfma<HM>(kf, qf[p][i], st[b]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
         if (c + WAVES < c1) request_k(coming);
         __builtin_amdgcn_sched_barrier(0);
-        float cm = -INFINITY;
+        // scores of keys that a row does not see, where the tile has some
+        if (j0 + 32 > end || j0 + 31 > rg.before - (!ONE && a.parents ? 1 : 0) || (a.window > 0 && rg.before + it.cnt - 1 - j0 >= a.window && j0 + 32 > a.first)) {
 #pragma unroll
-        for (int b = 0; b < 2; b++)
+            for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int key = j0 + b * 16 + 4 * q + i;
-                int at = key; bool ok = key < end;
-                if (!ONE && a.parents) {
-                    const int n = key - rg.before, d = __shfl(depth, n & 63);
-                    if (n >= 0) { at = rg.before + d; ok = ok && (seen >> (n & 63) & 1); }
-                } else ok = ok && key <= pos;
-                if (a.window > 0) ok = ok && (pos - at < a.window || at < a.first);
-                st[b][i] = ok ? st[b][i] * a.scale_log2 : -INFINITY;
-                cm = fmaxf(cm, st[b][i]);
+                for (int i = 0; i < 4; i++) {
+                    const int key = j0 + b * 16 + 4 * q + i;
+                    int at = key; bool ok = key < end;
+                    if (!ONE && a.parents) {
+                        const int n = key - rg.before, d = __shfl(depth, n & 63);
+                        if (n >= 0) { at = rg.before + d; ok = ok && (seen >> (n & 63) & 1); }
+                    } else ok = ok && key <= pos;
+                    if (a.window > 0) ok = ok && (pos - at < a.window || at < a.first);
+                    if (!ok) st[b][i] = -INFINITY;
+                }
+        }
+        // Weights from a reference, exp2(s - m): a row's first maximum in this wave, which moves, with what was summed so far, when a lane's sum gets out of the numbers' range (f16 ends at
+        // 2^16, bf16 and 32 bits are far from their end), and until the row has seen its first key.  NaN scores move nothing and are in the sums.
+        u32x4 pf[NP];
+        float hs = 0.0f;
+        auto weigh = [&]() {
+            hs = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 1][2 * (e & 1)], scale, -base)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 1][2 * (e & 1) + 1], scale, -base));
+                const uint32_t w = kv_pack<HM>(p0, p1);
+                pf[0][e] = w;
+                if constexpr (NP == 2) { pf[1][e] = kv_rest(p0, p1, w); hs += p0 + p1; }
+                else hs = kv_sum2<HM>(w, hs);
             }
-        cm = fmaxf(cm, __shfl_xor(cm, 16)); cm = fmaxf(cm, __shfl_xor(cm, 32));
-        const float mn = fmaxf(m, cm), base = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(m - base);
-        m = mn; l *= alpha;
-        u32x4 pf[PP];
+        };
+        weigh();
+        if (__any(hs > most)) {
+            float t = st[0][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) t = fmaxf(t, st[i >> 2][i & 3]);
+            t = fmaxf(t, __shfl_xor(t, 16)); t = fmaxf(t, __shfl_xor(t, 32));
+            const float mn = fmaxf(m, t * scale);
+            base = mn == -INFINITY ? 0.0f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - base);
+            m = mn; l *= f; most = mn == -INFINITY ? -1.0f : HM ? 8192.0f : 1073741824.0f;
+#pragma unroll
+            for (int j = 0; j < DIM / 16; j++) acc[j] *= f;
+            weigh();
+        }
+        l += hs;
+        constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;
+        // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys.
+        const bool look = !ONE && it.cnt > 1;
         uint32_t vis[4];                                      // ones where the row sees the key, as a fragment
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float s0 = st[e >> 1][2 * (e & 1)], s1 = st[e >> 1][2 * (e & 1) + 1];
-            const float p0 = __builtin_amdgcn_exp2f(s0 - base), p1 = __builtin_amdgcn_exp2f(s1 - base);
-            l += p0 + p1;
-            pf[0][e] = kv_pack<HM>(p0, p1);
-            if constexpr (PP == 2) pf[1][e] = kv_rest(p0, p1, pf[0][e]);
-            vis[e] = (s0 == -INFINITY ? 0u : (HM ? 0x3C00u : 0x3F80u)) | (s1 == -INFINITY ? 0u : (HM ? 0x3C000000u : 0x3F800000u));
-        }
-        if (__any(alpha != 1.0f)) {
-#pragma unroll
-            for (int j = 0; j < DIM / 16; j++) acc[j] *= alpha;
-        }
-        constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;
-        // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys: nothing to do, but for an
-        // infinity (16-bit pages hold them) and a weight whose second piece is 0 or negative.
-        const bool look = (FMT == 0 && PP == 2) || (!ONE && it.cnt > 1);
+        for (int e = 0; e < 4; e++) vis[e] = (st[e >> 1][2 * (e & 1)] == -INFINITY ? 0u : UNIT) | (st[e >> 1][2 * (e & 1) + 1] == -INFINITY ? 0u : UNIT << 16);
 #pragma unroll
         for (int g = 0; g < GROUPS; g++)
 #pragma unroll
@@ -235,7 +253,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
                         vf = keep;
                     }
 #pragma unroll
-                    for (int p = PP - 1; p >= 0; p--) acc[j] = kvs_mfma<HM>(vf, pf[p], acc[j]);
+                    for (int p = NP - 1; p >= 0; p--) acc[j] = kvs_mfma<HM>(vf, pf[p], acc[j]);
                 }
             }
         __builtin_amdgcn_sched_barrier(0);
@@ -251,11 +269,12 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     float top = -INFINITY, den = 0.0f;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) top = fmaxf(top, ml[w * 16 + row]);
-    const float base = top == -INFINITY ? 0.0f : top;
+    base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) den += dl[w * 16 + row] * __builtin_amdgcn_exp2f(ml[w * 16 + row] - base);
     const float f = __builtin_amdgcn_exp2f(m - base);
     float* mine = kvs_lds_ + (wave * 16 + row) * VS;
+    if (wave < c1 - c0)
 #pragma unroll
     for (int j = 0; j < DIM / 16; j++)
 #pragma unroll
@@ -264,11 +283,12 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     __syncthreads();
     const bool whole = it.nsplit == 1;
     float* wo = a.ws + (size_t)blockIdx.x * 16 * DIM;
+    const int had = min(WAVES, c1 - c0);                      // waves that had a tile
     for (int i = tid; i < rows * (DIM / 4); i += 64 * WAVES) {
         const int rr = i / (DIM / 4), d = (i - rr * (DIM / 4)) * 4;
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
+#pragma unroll 4
+        for (int w = 0; w < had; w++) {
             const float4 x = *reinterpret_cast<const float4*>(kvs_lds_ + (w * 16 + rr) * VS + d);
             s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
         }

@@ -78,11 +78,8 @@ def check(got, q, cache, fmt, states, counts, scale=None, window=0, first=0, tre
         k, v = stored_rows(cache, s, fmt)
         see = visible(s.seq_len - n, n, window, first, None if trees is None else trees[i])
         out, mean, size = attend(q[r:r + n].double(), k, v, see, scale)
-        # weights are f16 over f16 pages, else bf16, one piece of it in tiles of rows when q is bf16; half a step each.  Two pieces leave half a step of the second, 2^-8 of 2^-8.
-        if q.dtype == torch.float16:
-            weight = 2.0 ** -11 if native else 2.0 ** -16
-        else:
-            weight = 2.0 ** -8 if n * (heads // k.shape[1]) > 16 else 2.0 ** -16
+        # weights are f16 over f16 pages, else bf16, one piece of it when q is bf16; half a step each.  Two pieces leave half a step of the second, 2^-8 of 2^-8.
+        weight = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11 if native else 2.0 ** -16
         tol = tolerance(out, mean, size, dim, s.seq_len, q.dtype, weight)
         # 32 bits end at 2^-126: a weight under it is 0 (off by less than 2^-126 of its |v|), and so is a product of a weight and a value (off by less than 2^-126), for every key
         tol = tol + s.seq_len * 2.0 ** -126 * (v[v.isfinite()].abs().max() + 1)
