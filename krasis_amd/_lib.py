@@ -277,7 +277,7 @@ def load_library() -> C.CDLL:
     i64, sz = C.c_int64, C.c_size_t
     lib.kr_kv_plan.argtypes = [ci, ci, ci, vp, vp, vp, vp, vp, sz, C.POINTER(sz)]
     lib.kr_kv_write.argtypes = lib.kr_kv_read.argtypes = [vp, vp, vp, vp, vp, vp, ci, vp]
-    lib.kr_kv_attend_workspace.argtypes = [vp, vp, ci, ci, ci, ci, C.POINTER(sz)]
+    lib.kr_kv_attend_workspace.argtypes = [vp, vp, ci, ci, ci, ci, ci, C.POINTER(sz)]
     lib.kr_kv_attend.argtypes = [vp, vp, vp, vp, i64, i64, vp, ci, ci, cf, ci, ci, vp, vp, sz, vp]
     lib.kr_kv_move.argtypes = [vp, ci, ci, vp, vp, vp, vp]
     if hasattr(lib, "kr_serve_abi"):

@@ -88,10 +88,9 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
         if (rows < p.min_rows || rows > p.max_rows) continue;
         const int n = kv_tiles_ub(h.lens[b], cnt, kv_divisor((uint32_t)G), window, first, tree, p.bm, p.kt);
         const int64_t rt = (int64_t)kv_row_tiles(cnt, G, p.bm) * kv_heads;
-        if (cnt > 1) p.one = false;
         seqs.push_back({n, rt}); total += rt * n; whole += rt; longest = n > longest ? n : longest;
     }
-    p.items = whole; p.units = 0; p.split = p.few = false; p.one = !tree; p.tps = longest > 0 ? longest : 1;
+    p.items = whole; p.units = 0; p.split = p.few = false; p.tps = longest > 0 ? longest : 1;
     if (seqs.empty()) return;
     auto items = [&](int tps) { int64_t n = 0; for (const Seq& s : seqs) n += s.row_tiles * ((s.tiles + tps - 1) / tps); return n; };
     if (whole < 4ll * hold) {
@@ -116,11 +115,14 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
     p.few = most <= 16;
     if (p.split) for (const Seq& s : seqs) if (s.tiles > p.tps) p.units += s.row_tiles * (p.few ? p.bm / 16 : p.bm);
 }
-void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, int window, int first, bool tree, Part* p) {
+void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, bool half, int window, int first, bool tree, Part* p) {
     const int G = heads / kv_heads;
     p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, 1, false, false, false};
     p[1] = Part{KV_STEP_BM + 1, INT32_MAX, KV_TILE_BM, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
-    divide(h, kv_heads, G, window, first, tree, KV_CUS, kv_step_waves(dim, fmt), 3, 3, p[0]);
+    bool one = !tree;
+    for (int b = 0; b < h.batch && one; b++) { const int64_t cnt = h.row0[b + 1] - h.row0[b]; one = cnt <= 1 || cnt * G > KV_STEP_BM; }
+    p[0].one = one;
+    divide(h, kv_heads, G, window, first, tree, KV_CUS, kv_step_waves(dim, fmt, half, one), 3, 3, p[0]);
     divide(h, kv_heads, G, window, first, tree, kv_tile_waves(dim) * KV_CUS, 1, 3, 4, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
@@ -195,13 +197,13 @@ extern "C" int kr_kv_read(const kr_kv_pages* p, const int* plan, const int* dev_
     return rows_call("kr_kv_read", p, plan, dev_plan, k, v, strides, dtype, stream, false);
 }
 
-extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int window, int keep_first, int tree, size_t* bytes) {
+extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int dtype, int window, int keep_first, int tree, size_t* bytes) {
     KvPages o;
     if (int rc = check_attend(p, plan, heads, window, keep_first, tree != 0, o)) return rc;
     if (!bytes) return kr_fail(KR_ERR_VALUE, "kr_kv_attend_workspace: null argument");
     const Plan h(plan);
     Part part[2];
-    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), window, clamp_first(h, window, keep_first), tree != 0, part);
+    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), dtype == KR_KV_F16, window, clamp_first(h, window, keep_first), tree != 0, part);
     *bytes = part_bytes(part[0], p->dim) + part_bytes(part[1], p->dim);
     return KR_OK;
 }
@@ -223,7 +225,7 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
     a.window = window; a.first = clamp_first(h, window, keep_first);
     a.scale_log2 = scale * 1.44269504088896340736f;
     Part part[2];
-    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), window, a.first, parents != nullptr, part);
+    parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), dtype == KR_KV_F16, window, a.first, parents != nullptr, part);
     const size_t b0 = part_bytes(part[0], p->dim), b1 = part_bytes(part[1], p->dim);
     if (workspace_bytes < b0 + b1 || ((b0 + b1) && (!workspace || misaligned(workspace)))) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: a workspace of %zu bytes for %zu", workspace_bytes, b0 + b1);
     if (part[0].items > INT32_MAX || part[1].items > INT32_MAX || part[0].units > INT32_MAX || part[0].shares > KV_MAX_SHARES || part[1].shares > KV_MAX_SHARES || part[1].units > INT32_MAX) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: %d rows are too many for one call", h.rows);
@@ -233,7 +235,7 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
     static int (*const tile[3])(const KvAttnArgs&, int, int, hipStream_t) = {kr_launch_kv_tile_16, kr_launch_kv_tile_8, kr_launch_kv_tile_4};
     for (int i = 1; i >= 0; i--) {                            // prompts first, they take longest
         if (!part[i].items) continue;
-        a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = kv_divisor((uint32_t)part[i].tps); a.items = (int)part[i].items; a.one = part[i].one;
+        a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = kv_divisor((uint32_t)part[i].tps); a.items = (int)part[i].items; a.whole = a.items / (8 * p->kv_heads) * (8 * p->kv_heads); a.one = part[i].one;
         a.ws = (float*)((char*)workspace + (i ? b0 : 0));
         if (int rc = launched("kr_kv_attend", i ? tile[fmt](a, p->dim, half, st) : step[fmt](a, p->dim, half, st))) return rc;
         if (part[i].split)

@@ -40,7 +40,7 @@ struct KvAttnArgs {
     float scale_log2;                  // scale * log2(e): scores are kept in units of log 2
     int min_rows, max_rows;            // the sequences of this launch: those whose new rows times G lie in between
     KvDiv tps;                         // key tiles a workgroup takes at most
-    int items, one;                    // one: no sequence of this launch has more than one new token, and there are no trees
+    int items, whole, one;                    // whole: items / (8 kv_heads) * (8 kv_heads); one: no sequence of this launch has more than one new token, and there are no trees
     float* ws;                         // partial results of sequences that are split: [item][KV_BM rows][dim] sums, then [item][rows][2] maximum and denominator
 };
 
@@ -60,7 +60,10 @@ constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step_dev.h
 constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile_dev.h
 __host__ __device__ constexpr int kv_tile_waves(int dim) { return dim <= 128 ? 2 : 1; }      // that a SIMD holds of the latter, by registers and LDS
-__host__ __device__ constexpr int kv_step_waves(int dim, int fmt) { return dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8; }      // of a workgroup in kr_kv_step_dev.h, one a CU: by registers
+// waves of a workgroup in kr_kv_step_dev.h, one workgroup a CU: by registers.  half: f16 queries (two pieces over pages that become bf16); one: every sequence has one new token
+__host__ __device__ constexpr int kv_step_waves(int dim, int fmt, bool half, bool one) {
+    return !one ? (dim <= 128 ? 8 : 4) : dim == 64 || (dim == 96 && fmt == 0) || (dim == 128 && fmt == 2 && !half) ? 16 : dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8;
+}
 constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
 
 // ---- the division of a launch into items, the same on the host (how many) and on the device (which one)

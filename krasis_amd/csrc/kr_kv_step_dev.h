@@ -10,6 +10,7 @@
 #pragma once
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
+#include <type_traits>
 
 template <int DIM> struct KvsCols { static constexpr int C = DIM == 96 ? 2 : DIM == 192 ? 4 : DIM / 16, GROUPS = DIM / (16 * C); };      // columns of V a lane holds: groups of 16 C
 constexpr int kvs_lds(int dim, int waves) { return (waves * 16 * (dim + 4) + waves * 32 + 32) * (int)sizeof(float); }
@@ -40,15 +41,23 @@ template <bool H> __device__ __forceinline__ kv_f4 kvs_mfma(u32x4 x, u32x4 y, kv
 
 // HQ: q and out are f16.  Products are f16 where the pages are f16 too, else bf16.  ONE: every sequence of the launch has one new token and no tree, so that its rows see the same keys.
 template <int DIM, int FMT, bool HQ, bool ONE>
-__global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DIM, FMT) / 4) kr_kv_step_kernel(const KvAttnArgs a) {
-    constexpr int WAVES = kv_step_waves(DIM, FMT);
+__global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step_waves(DIM, FMT, HQ, ONE) / 4) kr_kv_step_kernel(const KvAttnArgs a) {
+    constexpr int WAVES = kv_step_waves(DIM, FMT, HQ, ONE);
     constexpr bool HM = HQ && FMT == 0;                       // f16 products
     constexpr int NP = HQ && !HM ? 2 : 1;                     // bf16 pieces of an f16 query and of its weights
     constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, U = DIM / 32, KB = DIM / 4 * BITS / 8, KW = KB / 4;
     constexpr int C = KvsCols<DIM>::C, GROUPS = KvsCols<DIM>::GROUPS, VB = C * BITS / 8, VW = VB < 4 ? 1 : VB / 4;
     constexpr int NB = DIM == 64 || DIM == 128 ? 1 : 2;       // blocks of 32 channels that a quarter of a row meets
     extern __shared__ float kvs_lds_[];
-    const KvItem it = kv_item<true>(a, blockIdx.x, 16, KV_STEP_KT, KvDiv{});
+    // Workgroups go round the eight XCDs in turn, and heads lie side by side in a token's row: all heads of a share go to one XCD, whose L2 then fetches a line that two of them have parts
+    // of (64 bytes of a head at four bits, the scales of any) once.  32 x 8192 tokens at four bits 56 -> 36 us.
+    int idx = blockIdx.x;
+    if (const int whole = a.whole; idx < whole) {
+        uint32_t head;
+        const uint32_t group = kv_div((uint32_t)idx >> 3, a.kv_heads, head) * 8 + (idx & 7);
+        idx = (int)(group * a.kv_heads.d + head);
+    }
+    const KvItem it = kv_item<true>(a, idx, 16, KV_STEP_KT, KvDiv{});
     if (it.b < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 15, q = lane >> 4;
     const KvRange rg = kv_range(a, it, 16, KV_STEP_KT);
@@ -88,13 +97,17 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
         }
     }
 
-    // A wave asks for the next tile's keys when it has used this one's, for its values likewise, and for slots a tile earlier still: one set of registers for each, so that more waves
+    // A wave asks for the next tile's keys when it has used this one's, for its values likewise, and for pages a tile earlier still: one set of registers for each, so that more waves
     // than with two sets have a tile on its way.
     uint32_t kn[2][KW], vn[8][GROUPS][VW]; uint32_t ksn[2][NB], vsn[8][GROUPS];
-    auto places = [&](int c) {                                // of key `lane` of a tile, in units of 16 bytes; keys no row sees give way to one that is seen
+    // where key `lane` of a tile lies: its page is asked for a tile before the place is formed; keys no row sees give way to one that is seen
+    uint32_t page = 0, in = 0;
+    auto find = [&](int c) {
+        c = min(c, c1 - 1);
         const int j = (c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept)) + (lane & 31);
-        return kv_slot(a.p, table, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1))) * a.p.row16;
+        page = (uint32_t)table[kv_page(a.p, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1)), in)];
     };
+    auto place = [&]() { return (page * a.p.page.d + in) * a.p.row16; };      // in units of 16 bytes
     auto request_k = [&](uint32_t s) {
         uint32_t at[2];
 #pragma unroll
@@ -128,16 +141,8 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     kv_f4 acc[DIM / 16];
 #pragma unroll
     for (int j = 0; j < DIM / 16; j++) acc[j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t next = 0;
-    if (c0 + wave < c1) {
-        const uint32_t s = places(c0 + wave);
-        if (c0 + wave + WAVES < c1) next = places(c0 + wave + WAVES);
-        request_k(s); request_v(s);
-    }
-    for (int c = c0 + wave; c < c1; c += WAVES) {
+    auto tile = [&](int c, auto MORE) {                       // MORE: the wave has another tile
         const int j0 = c < rg.kept ? 32 * c : rg.start + 32 * (c - rg.kept), end = c < rg.kept ? min(a.first, rg.hi) : rg.hi;
-        const uint32_t coming = next;
-        if (c + 2 * WAVES < c1) next = places(c + 2 * WAVES);
         kv_f4 st[2];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -157,7 +162,8 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (c + WAVES < c1) request_k(coming);
+        uint32_t coming = 0;
+        if constexpr (MORE) { coming = place(); request_k(coming); }
         __builtin_amdgcn_sched_barrier(0);
         // scores of keys that a row does not see, where the tile has some
         if (j0 + 32 > end || j0 + 31 > rg.before - (!ONE && a.parents ? 1 : 0) || (a.window > 0 && rg.before + it.cnt - 1 - j0 >= a.window && j0 + 32 > a.first)) {
@@ -257,8 +263,17 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
                 }
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (c + WAVES < c1) request_v(coming);
+        if constexpr (MORE) { request_v(coming); find(c + 2 * WAVES); }
         __builtin_amdgcn_sched_barrier(0);
+    };
+    if (c0 + wave < c1) {
+        int c = c0 + wave;
+        find(c);
+        const uint32_t s = place();
+        request_k(s); request_v(s);
+        find(c + WAVES);
+        for (; c + WAVES < c1; c += WAVES) tile(c, std::integral_constant<bool, true>());
+        tile(c, std::integral_constant<bool, false>());
     }
     // ---- the waves' states meet: [waves][16][DIM + 4] sums | [waves][16] maxima | [waves][16] denominators | [16] maximum | [16] denominator
     constexpr int VS = DIM + 4;
@@ -282,7 +297,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
     if (tid < 16) { mt[tid] = top; dt[tid] = den; }
     __syncthreads();
     const bool whole = it.nsplit == 1;
-    float* wo = a.ws + (size_t)blockIdx.x * 16 * DIM;
+    float* wo = a.ws + (size_t)idx * 16 * DIM;
     const int had = min(WAVES, c1 - c0);                      // waves that had a tile
     for (int i = tid; i < rows * (DIM / 4); i += 64 * WAVES) {
         const int rr = i / (DIM / 4), d = (i - rr * (DIM / 4)) * 4;
@@ -300,13 +315,13 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT), kv_step_waves(DI
         } else *reinterpret_cast<float4*>(wo + rr * DIM + d) = s;
     }
     if (!whole && tid < 16) {
-        float* st = a.ws + (size_t)a.items * 16 * DIM + ((size_t)blockIdx.x * 16 + tid) * 2;
+        float* st = a.ws + (size_t)a.items * 16 * DIM + ((size_t)idx * 16 + tid) * 2;
         st[0] = mt[tid]; st[1] = dt[tid];
     }
 }
 
 template <int DIM, int FMT, bool HQ, bool ONE> static int kvs_launch(const KvAttnArgs& a, hipStream_t st) {
-    constexpr int waves = kv_step_waves(DIM, FMT);
+    constexpr int waves = kv_step_waves(DIM, FMT, HQ, ONE);
     constexpr size_t lds = kvs_lds(DIM, waves);
     if (lds > 65536 && kr_lds_optin((const void*)kr_kv_step_kernel<DIM, FMT, HQ, ONE>, lds)) return 1;
     hipLaunchKernelGGL((kr_kv_step_kernel<DIM, FMT, HQ, ONE>), dim3(a.items), dim3(64 * waves), lds, st, a);

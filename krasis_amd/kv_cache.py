@@ -375,11 +375,11 @@ class KVBatch:
             out = torch.empty((self.rows, heads, d), dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"out: contiguous {q.dtype} {tuple(q.shape)} on {q.device}, aligned to 16 bytes")
-        pages, key = self._layer(layer), (heads, window, keep_first, parents is not None)
+        pages, key = self._layer(layer), (heads, q.dtype, window, keep_first, parents is not None)
         need = self._need.get(key)
         if need is None:
             size = ctypes.c_size_t()
-            _lib.check(self._lib.kr_kv_attend_workspace(pages, self._plan[0], heads, window, keep_first, int(parents is not None), ctypes.byref(size)))
+            _lib.check(self._lib.kr_kv_attend_workspace(pages, self._plan[0], heads, _ROWS[q.dtype], window, keep_first, int(parents is not None), ctypes.byref(size)))
             self._need[key] = need = size.value
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None      # of this call alone: two streams, or two graphs, never share one
         self._call(self._lib.kr_kv_attend, pages, *self._plan, q.data_ptr(), qt, qh, out.data_ptr(), _ROWS[q.dtype], heads, d ** -0.5 if scale is None else scale,

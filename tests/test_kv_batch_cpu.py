@@ -168,7 +168,7 @@ def test_workspaces_grow_with_the_shares():
 
     def need(st, cnt, heads, window=0, tree=0):
         plan = plan_of(cache, st, cnt)
-        _lib.check(_lib.load_library().kr_kv_attend_workspace(ctypes.byref(pages), plan.data_ptr(), heads, window, 4, tree, ctypes.byref(size)))
+        _lib.check(_lib.load_library().kr_kv_attend_workspace(ctypes.byref(pages), plan.data_ptr(), heads, 0, window, 4, tree, ctypes.byref(size)))
         return size.value
     assert need([short], [1], 16) == 0 and need([long], [1], 16) > 0 and need([long], [40], 16, tree=1) > 0
     assert need([long], [1], 16, window=32) == 0
