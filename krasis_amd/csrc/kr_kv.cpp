@@ -76,10 +76,11 @@ int rows_call(const char* what, const kr_kv_pages* p, const int* plan, const int
 
 // one launch's share of a call: the sequences whose rows (new tokens x heads of a group) lie in a range
 struct Part { int min_rows, max_rows, bm, kt, tps; int64_t items, units; int shares; bool split, few, one; };
-// How many key tiles a workgroup takes.  `hold` workgroups are on the chip at once and `side` tiles are worked on side by side in one, so a launch lasts rounds * (tiles / side + what it
-// takes to begin and to end, `extra`), and `join` more when shares have to be joined (all in the time of a tile); the cheapest number of rounds up to four is taken.  More row tiles than
-// that fill the chip evenly by themselves.
-void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int hold, int side, int extra, int join, Part& p) {
+// How many key tiles a workgroup takes.  A workgroup works on `side` tiles side by side, `deep` workgroups share a CU's time.  With k workgroups a CU a launch lasts k tiles' time for every
+// `side` tiles of a share, what it takes to begin and to end (`extra`) for every `deep` workgroups, and `join` more when shares have to be joined (all in the time of a tile): the cheapest
+// number up to 4 * deep is taken.  More row tiles than that fill the chip evenly by themselves.
+void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int deep, int side, int extra, int join, Part& p) {
+    constexpr int hold = KV_CUS;
     struct Seq { int tiles; int64_t row_tiles; };
     std::vector<Seq> seqs;
     int64_t total = 0, whole = 0; int longest = 0;
@@ -93,14 +94,14 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
     p.items = whole; p.units = 0; p.split = p.few = false; p.tps = longest > 0 ? longest : 1;
     if (seqs.empty()) return;
     auto items = [&](int tps) { int64_t n = 0; for (const Seq& s : seqs) n += s.row_tiles * ((s.tiles + tps - 1) / tps); return n; };
-    if (whole < 4ll * hold) {
+    auto cost = [&](int64_t k, int tiles) { return k * ((tiles + side - 1) / side) + (k + deep - 1) / deep * extra; };
+    if (whole < 4ll * deep * hold) {
         const int least = std::max(side, (longest + KV_MAX_SHARES - 1) / KV_MAX_SHARES);
-        int64_t best = ((whole + hold - 1) / hold) * ((longest + side - 1) / side + extra);
-        for (int64_t k = (whole + hold - 1) / hold; k <= 4; k++) {
-            int lo = std::max(least, (int)(total / (k * hold))), hi = longest;      // the smallest share whose items fit into k rounds
+        int64_t k = (whole + hold - 1) / hold, best = cost(k, longest);
+        for (; k <= 4 * deep; k++) {
+            int lo = std::max(least, (int)(total / (k * hold))), hi = longest;      // the smallest share whose items fit
             while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (items(mid) <= k * hold) hi = mid; else lo = mid + 1; }
-            const int64_t cost = k * ((lo + side - 1) / side + extra) + join;
-            if (lo < longest && cost < best) { best = cost; p.tps = lo; }
+            if (lo < longest && cost(k, lo) + join < best) { best = cost(k, lo) + join; p.tps = lo; }
         }
     }
     int most = 1;
@@ -122,8 +123,8 @@ void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, bool hal
     bool one = !tree;
     for (int b = 0; b < h.batch && one; b++) { const int64_t cnt = h.row0[b + 1] - h.row0[b]; one = cnt <= 1 || cnt * G > KV_STEP_BM; }
     p[0].one = one;
-    divide(h, kv_heads, G, window, first, tree, KV_CUS, kv_step_waves(dim, fmt, half, one), 3, 3, p[0]);
-    divide(h, kv_heads, G, window, first, tree, kv_tile_waves(dim) * KV_CUS, 1, 3, 4, p[1]);
+    divide(h, kv_heads, G, window, first, tree, 1, kv_step_waves(dim, fmt, half, one), 3, 3, p[0]);
+    divide(h, kv_heads, G, window, first, tree, kv_tile_waves(dim), 1, 6, 5, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
 
@@ -197,7 +198,7 @@ extern "C" int kr_kv_read(const kr_kv_pages* p, const int* plan, const int* dev_
     return rows_call("kr_kv_read", p, plan, dev_plan, k, v, strides, dtype, stream, false);
 }
 
-extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int dtype, int window, int keep_first, int tree, size_t* bytes) {
+static int attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int dtype, int window, int keep_first, int tree, size_t* bytes) {
     KvPages o;
     if (int rc = check_attend(p, plan, heads, window, keep_first, tree != 0, o)) return rc;
     if (!bytes) return kr_fail(KR_ERR_VALUE, "kr_kv_attend_workspace: null argument");
@@ -208,7 +209,7 @@ extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int
     return KR_OK;
 }
 
-extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* dev_plan, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int dtype, int heads, float scale,
+static int attend(const kr_kv_pages* p, const int* plan, const int* dev_plan, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int dtype, int heads, float scale,
                             int window, int keep_first, const int* parents, void* workspace, size_t workspace_bytes, void* stream) {
     KvAttnArgs a{};
     if (int rc = check_attend(p, plan, heads, window, keep_first, parents != nullptr, a.p)) return rc;
@@ -242,6 +243,17 @@ extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* de
             if (int rc = launched("kr_kv_attend", kr_launch_kv_join(a, p->dim, part[i].bm, part[i].kt, (int)part[i].units, part[i].few, half, st))) return rc;
     }
     return KR_OK;
+}
+
+// no exception leaves a C entry: the division of a call keeps a list of its sequences
+extern "C" int kr_kv_attend_workspace(const kr_kv_pages* p, const int* plan, int heads, int dtype, int window, int keep_first, int tree, size_t* bytes) {
+    try { return attend_workspace(p, plan, heads, dtype, window, keep_first, tree, bytes); }
+    catch (const std::exception& x) { return kr_fail(KR_ERR_STATE, "kr_kv_attend_workspace: %s", x.what()); }
+}
+extern "C" int kr_kv_attend(const kr_kv_pages* p, const int* plan, const int* dev_plan, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int dtype, int heads, float scale,
+                            int window, int keep_first, const int* parents, void* workspace, size_t workspace_bytes, void* stream) {
+    try { return attend(p, plan, dev_plan, q, q_token_stride, q_head_stride, out, dtype, heads, scale, window, keep_first, parents, workspace, workspace_bytes, stream); }
+    catch (const std::exception& x) { return kr_fail(KR_ERR_STATE, "kr_kv_attend: %s", x.what()); }
 }
 
 extern "C" int kr_kv_move(const kr_kv_pages* p, int layers, int n_seq, const int* dev_start, const int* dev_src, const int* dev_dst, void* stream) {

@@ -45,25 +45,40 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     const int* table = a.s.pages + it.page0;
     const float scale = fmaxf(fabsf(a.scale_log2), 1.1754944e-38f);      // its sign goes into the queries: scores that are not seen are -infinity before it, too
 
-    int tk, pos; uint64_t seen;
-    uint64_t all = 0;
-    if (a.parents) {
-        all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
-        if (tid < KV_MAX_TREE) Dp[tid] = __popcll(all) - 1;
-    }
+    auto first_key = [&](int c) { return c < rg.kept ? KT * c : rg.start + KT * (c - rg.kept); };
+    auto page_of = [&](int c, int k, uint32_t& in) {          // keys no row sees give way to one that is seen
+        const int j = first_key(c) + k;
+        return kv_page(a.p, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1)), in);
+    };
+    auto place = [&](int c, int k) {
+        uint32_t in;
+        const uint32_t n = page_of(c, k, in);
+        return ((uint32_t)table[n] * a.p.page.d + in) * a.p.row16;
+    };
+    // What depends on nothing is asked for first: the pages of the first eight tiles' keys, the queries, the drafts' parents.
+    uint32_t page[NS * KT / 256], in[NS * KT / 256];
+    if (c0 < c1)
+#pragma unroll
+        for (int i = 0; i < NS * KT / 256; i++) page[i] = (uint32_t)table[page_of(min(c0 + 4 * i + (tid >> 6), c1 - 1), lane, in[i])];
     u32x4 qf[NP][KS];
+    const int r = min(rw + col, rows - 1), tk = (int)kv_div((uint32_t)r, a.G);
     {
-        const int r = min(rw + col, rows - 1);
-        tk = (int)kv_div((uint32_t)r, a.G); pos = rg.before + tk; seen = 0;
-        if (a.parents) {
-            seen = (uint64_t)__shfl((uint32_t)(all >> 32), tk) << 32 | __shfl((uint32_t)all, tk);
-            pos = rg.before + __popcll(seen) - 1;
-        }
         const uint16_t* qp = a.q + (size_t)(it.row0 + tk) * a.q_tok + (size_t)(it.kvh * G + r - tk * G) * a.q_head + 8 * h;
+#pragma unroll
+        for (int i = 0; i < KS; i++) qf[0][i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
+    }
+    int pos = rg.before + tk; uint64_t seen = 0;
+    if (a.parents) {
+        const uint64_t all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
+        if (tid < KV_MAX_TREE) Dp[tid] = __popcll(all) - 1;
+        seen = (uint64_t)__shfl((uint32_t)(all >> 32), tk) << 32 | __shfl((uint32_t)all, tk);
+        pos = rg.before + __popcll(seen) - 1;
+    }
+    auto queries = [&]() {                                    // as they enter the products: the scale's sign, two pieces of f16 where the products are bf16
         const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * i) ^ sign;
+            const u32x4 x = qf[0][i] ^ sign;
             if constexpr (NP == 1) qf[0][i] = x;
             else {
 #pragma unroll
@@ -75,16 +90,6 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
                 }
             }
         }
-    }
-    auto first_key = [&](int c) { return c < rg.kept ? KT * c : rg.start + KT * (c - rg.kept); };
-    auto page_of = [&](int c, int k, uint32_t& in) {          // keys no row sees give way to one that is seen
-        const int j = first_key(c) + k;
-        return kv_page(a.p, (uint32_t)(j < rg.lo && j >= a.first ? rg.lo : min(j, rg.hi - 1)), in);
-    };
-    auto place = [&](int c, int k) {
-        uint32_t in;
-        const uint32_t n = page_of(c, k, in);
-        return ((uint32_t)table[n] * a.p.page.d + in) * a.p.row16;
     };
     // this thread's chunks: row of the tile, place in the row
     u32x4 kn[PT], vn[PT]; uint32_t ksn[PT], vsn[PT], off[PT], coming[PT];
@@ -274,23 +279,22 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     if (c0 < c1) {
         if (tid == 0) *Odd = 0;
 #pragma unroll
-        for (int i = 0; i < NS * KT / 256; i++) {
-            const int c = c0 + 4 * i + (tid >> 6);
-            Sl[(c & (NS - 1)) * KT + lane] = place(min(c, c1 - 1), lane);
-        }
+        for (int i = 0; i < NS * KT / 256; i++) Sl[((c0 + 4 * i + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[i] * a.p.page.d + in[i]) * a.p.row16;
         __syncthreads();
         places(c0, off); places(c0 + 1, coming);
+        u32x4 k2[PT]; uint32_t ks2[PT];
 #pragma unroll
-        for (int j = 0; j < PT; j++) { request(kb, ksb, kn, ksn, off[j], j); request(vb, vsb, vn, vsn, off[j], j); }
+        for (int j = 0; j < PT; j++) { request(kb, ksb, kn, ksn, off[j], j); request(vb, vsb, vn, vsn, off[j], j); request(kb, ksb, k2, ks2, coming[j], j); }
+        queries();
         if (c0 < gf || c0 >= gt) look();
+        places(c0 + 2, off);
 #pragma unroll
         for (int j = 0; j < PT; j++) {
             commit(Ks + (c0 & 1) * KT * LDK, LDK, kn, ksn, j); commit(Vs + (c0 & 1) * KT * LDV, LDV, vn, vsn, j);
-            request(kb, ksb, kn, ksn, coming[j], j); request(vb, vsb, vn, vsn, coming[j], j);
+            request(vb, vsb, vn, vsn, coming[j], j); request(kb, ksb, kn, ksn, off[j], j);
         }
-        places(c0 + 2, off);
 #pragma unroll
-        for (int j = 0; j < PT; j++) { commit(Ks + ((c0 + 1) & 1) * KT * LDK, LDK, kn, ksn, j); request(kb, ksb, kn, ksn, off[j], j); }
+        for (int j = 0; j < PT; j++) commit(Ks + ((c0 + 1) & 1) * KT * LDK, LDK, k2, ks2, j);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RING; i++) kr[i] = key(keys_at(c0, 0), i);
@@ -298,13 +302,12 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
 #pragma unroll
         for (int i = 0; i < RING; i++) kr[i] = key(keys_at(c0, 1), i);
         if (c0 < wf || c0 >= wt) mask(c0, 0, sa);
-        uint32_t page = 0, in = 0;
         // A tile: the scores of its first half are in sa, masked; its values and the next tile's keys are in LDS behind the barrier.
         for (int c = c0; c < c1; c++) {
             __syncthreads();
             // the places of tiles c + 8 .. c + 11: their pages are asked for, and a tile later they take the place of tiles whose keys have all been asked for
             const int turn = (c - c0) & 3;
-            if (turn == 0) page = (uint32_t)table[page_of(min(c + NS + (tid >> 6), c1 - 1), lane, in)];
+            if (turn == 0) page[0] = (uint32_t)table[page_of(min(c + NS + (tid >> 6), c1 - 1), lane, in[0])];
             scores(c, 1, sb, sa, c, 0, yes());
             if (c < wf || c >= wt) mask(c, 1, sb);
             settle(sa);
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
             settle(sb);
             places(c + 3, coming);
             sums(c, 1, c + 1, 1, yes());
-            if (turn == 1) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page * a.p.page.d + in) * a.p.row16;
+            if (turn == 1) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[0] * a.p.page.d + in[0]) * a.p.row16;
         }
         __syncthreads();
         if (*Odd) {                                           // the values that became 0 above: every row takes those that it sees
@@ -353,8 +356,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     }
     {
         l += __shfl_xor(l, 32);
-        const int r = rw + col;
-        if (r >= rows) return;
+    if (rw + col >= rows) return;
         if (it.nsplit == 1) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint16_t* op = a.out + ((size_t)(it.row0 + tk) * a.heads + it.kvh * G + r - tk * G) * DIM + 4 * h;
