@@ -67,10 +67,10 @@ int rows_call(const char* what, const kr_kv_pages* p, const int* plan, const int
     if (!s.rows) return KR_OK;
     if (!dev || !k || !v || !strides || misaligned(k) || misaligned(v)) return kr_fail(KR_ERR_VALUE, "%s: rows must be aligned to 16 bytes", what);
     for (int i = 0; i < 4; i++) if (strides[i] % 8) return kr_fail(KR_ERR_VALUE, "%s: strides must be multiples of 8 elements", what);
-    if ((int64_t)s.rows * (p->kv_heads * p->dim / 8) > INT32_MAX - 256) return kr_fail(KR_ERR_VALUE, "%s: %d rows are too many for one call", what, s.rows);
+    if ((int64_t)s.rows * (p->kv_heads * p->dim / 8) > INT32_MAX - 4096) return kr_fail(KR_ERR_VALUE, "%s: %d rows are too many for one call", what, s.rows);
     a.slots = s.slots; a.rows = s.rows; a.k = (void*)k; a.v = (void*)v;
     a.k_tok = strides[0]; a.k_head = strides[1]; a.v_tok = strides[2]; a.v_head = strides[3];
-    a.kv_heads = p->kv_heads; a.dim = p->dim; a.format = p->format; a.half = dtype == KR_KV_F16;
+    a.per_row = kv_divisor((uint32_t)(p->kv_heads * p->dim / 8)); a.per_head = kv_divisor((uint32_t)(p->dim / 8)); a.format = p->format; a.half = dtype == KR_KV_F16;
     return launched(what, write ? kr_launch_kv_write(a, stream_of(stream)) : kr_launch_kv_read(a, stream_of(stream)));
 }
 
@@ -119,12 +119,16 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
 void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, bool half, int window, int first, bool tree, Part* p) {
     const int G = heads / kv_heads;
     p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, 1, false, false, false};
-    p[1] = Part{KV_STEP_BM + 1, INT32_MAX, KV_TILE_BM, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
+    // Eight waves share what brings a tile to LDS where two of them fit on a SIMD and some sequence has rows for more than four.
+    int64_t most = 0;
+    for (int b = 0; b < h.batch; b++) most = std::max(most, (int64_t)(h.row0[b + 1] - h.row0[b]) * G);
+    const int waves = (dim == 96 || dim == 128) && most > 128 ? 8 : 4;
+    p[1] = Part{KV_STEP_BM + 1, INT32_MAX, 32 * waves, KV_TILE_KT, 0, 0, 0, 1, false, false, false};
     bool one = !tree;
     for (int b = 0; b < h.batch && one; b++) { const int64_t cnt = h.row0[b + 1] - h.row0[b]; one = cnt <= 1 || cnt * G > KV_STEP_BM; }
     p[0].one = one;
     divide(h, kv_heads, G, window, first, tree, 1, kv_step_waves(dim, fmt, half, one), 3, 3, p[0]);
-    divide(h, kv_heads, G, window, first, tree, kv_tile_waves(dim), 1, 6, 5, p[1]);
+    divide(h, kv_heads, G, window, first, tree, waves == 8 ? 1 : kv_tile_waves(dim), 1, 6, 5, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
 
@@ -233,12 +237,12 @@ static int attend(const kr_kv_pages* p, const int* plan, const int* dev_plan, co
     const int fmt = fmt_of(p->format), half = dtype == KR_KV_F16;
     hipStream_t st = stream_of(stream);
     static int (*const step[3])(const KvAttnArgs&, int, int, hipStream_t) = {kr_launch_kv_step_16, kr_launch_kv_step_8, kr_launch_kv_step_4};
-    static int (*const tile[3])(const KvAttnArgs&, int, int, hipStream_t) = {kr_launch_kv_tile_16, kr_launch_kv_tile_8, kr_launch_kv_tile_4};
+    static int (*const tile[3])(const KvAttnArgs&, int, int, int, hipStream_t) = {kr_launch_kv_tile_16, kr_launch_kv_tile_8, kr_launch_kv_tile_4};
     for (int i = 1; i >= 0; i--) {                            // prompts first, they take longest
         if (!part[i].items) continue;
         a.min_rows = part[i].min_rows; a.max_rows = part[i].max_rows; a.tps = kv_divisor((uint32_t)part[i].tps); a.items = (int)part[i].items; a.whole = a.items / (8 * p->kv_heads) * (8 * p->kv_heads); a.one = part[i].one;
         a.ws = (float*)((char*)workspace + (i ? b0 : 0));
-        if (int rc = launched("kr_kv_attend", i ? tile[fmt](a, p->dim, half, st) : step[fmt](a, p->dim, half, st))) return rc;
+        if (int rc = launched("kr_kv_attend", i ? tile[fmt](a, p->dim, half, part[i].bm / 32, st) : step[fmt](a, p->dim, half, st))) return rc;
         if (part[i].split)
             if (int rc = launched("kr_kv_attend", kr_launch_kv_join(a, p->dim, part[i].bm, part[i].kt, (int)part[i].units, part[i].few, half, st))) return rc;
     }

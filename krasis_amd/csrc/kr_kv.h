@@ -25,7 +25,7 @@ struct KvSeqs {
     int batch, rows;
 };
 
-struct KvRowsArgs { KvPages p; const int* slots; void *k, *v; long k_tok, k_head, v_tok, v_head; int rows, kv_heads, dim, format, half; };      // strides in elements; half: rows are f16
+struct KvRowsArgs { KvPages p; const int* slots; void *k, *v; long k_tok, k_head, v_tok, v_head; KvDiv per_row, per_head; int rows, format, half; };      // strides in elements; per_row, per_head: units of eight channels; half: rows are f16
 struct KvMoveArgs { uint8_t* base[4]; long layer_bytes[4]; int row_bytes[4]; const int *start, *src, *dst; int n_seq, layers; };
 
 struct KvAttnArgs {
@@ -47,18 +47,18 @@ struct KvAttnArgs {
 int kr_launch_kv_write(const KvRowsArgs& a, hipStream_t st);
 int kr_launch_kv_read(const KvRowsArgs& a, hipStream_t st);
 int kr_launch_kv_move(const KvMoveArgs& a, hipStream_t st);
-// by the width of the pages' numbers; half: q and out are f16
+// by the width of the pages' numbers; half: q and out are f16; waves: of a workgroup, 32 rows each
 int kr_launch_kv_step_16(const KvAttnArgs& a, int dim, int half, hipStream_t st);
 int kr_launch_kv_step_8(const KvAttnArgs& a, int dim, int half, hipStream_t st);
 int kr_launch_kv_step_4(const KvAttnArgs& a, int dim, int half, hipStream_t st);
-int kr_launch_kv_tile_16(const KvAttnArgs& a, int dim, int half, hipStream_t st);
-int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, hipStream_t st);
-int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, hipStream_t st);
+int kr_launch_kv_tile_16(const KvAttnArgs& a, int dim, int half, int waves, hipStream_t st);
+int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, int waves, hipStream_t st);
+int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, int waves, hipStream_t st);
 int kr_launch_kv_join(const KvAttnArgs& a, int dim, int bm, int kt, int units, int few, int half, hipStream_t st);
 constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 
 constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step_dev.h
-constexpr int KV_TILE_BM = 128, KV_TILE_KT = 64;     // and in kr_kv_tile_dev.h
+constexpr int KV_TILE_KT = 64;                       // keys of a tile in kr_kv_tile_dev.h; 32 rows a wave
 __host__ __device__ constexpr int kv_tile_waves(int dim) { return dim == 64 ? 3 : dim <= 128 ? 2 : 1; }      // that a SIMD holds of the latter, by registers and LDS
 // waves of a workgroup in kr_kv_step_dev.h, one workgroup a CU: by registers.  half: f16 queries (two pieces over pages that become bf16); one: every sequence has one new token
 __host__ __device__ constexpr int kv_step_waves(int dim, int fmt, bool half, bool one) {

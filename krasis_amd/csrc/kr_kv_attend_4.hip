@@ -3,4 +3,4 @@
 #include "kr_kv_tile_dev.h"
 
 int kr_launch_kv_step_4(const KvAttnArgs& a, int dim, int half, hipStream_t st) { return kvs_dim<2>(a, dim, half, st); }
-int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, hipStream_t st) { return kvt_dim<2>(a, dim, half, st); }
+int kr_launch_kv_tile_4(const KvAttnArgs& a, int dim, int half, int waves, hipStream_t st) { return kvt_dim<2>(a, dim, half, waves, st); }

@@ -3,4 +3,4 @@
 #include "kr_kv_tile_dev.h"
 
 int kr_launch_kv_step_8(const KvAttnArgs& a, int dim, int half, hipStream_t st) { return kvs_dim<1>(a, dim, half, st); }
-int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, hipStream_t st) { return kvt_dim<1>(a, dim, half, st); }
+int kr_launch_kv_tile_8(const KvAttnArgs& a, int dim, int half, int waves, hipStream_t st) { return kvt_dim<1>(a, dim, half, waves, st); }

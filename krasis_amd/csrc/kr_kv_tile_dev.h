@@ -24,12 +24,12 @@ template <bool H> __device__ __forceinline__ kv_f16 kvt_mfma(u32x4 x, u32x4 y, k
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(kv_b8, x), __builtin_bit_cast(kv_b8, y), c, 0, 0, 0);
 }
 
-template <int DIM, int FMT, bool HQ>
-__global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(const KvAttnArgs a) {
+template <int DIM, int FMT, bool HQ, int W>
+__global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv_tile_kernel(const KvAttnArgs a) {
     constexpr bool HM = HQ && FMT == 0;
     constexpr int NP = HQ && !HM ? 2 : 1;                     // bf16 pieces of an f16 query and of its weights
-    constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, CPR = DIM * BITS / 128, NCH = KT * CPR, PT = (NCH + 255) / 256, CD = 128 / BITS;      // chunks of 16 bytes, CD channels
-    constexpr int LDK = kvt_ldk(DIM), LDV = kvt_ldv(DIM), KS = DIM / 16, DB = DIM / 32, BM = 128, RING = 4, NS = KVT_PLACES;
+    constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, CPR = DIM * BITS / 128, NCH = KT * CPR, NT = 64 * W, PT = (NCH + NT - 1) / NT, CD = 128 / BITS;      // chunks of 16 bytes, CD channels
+    constexpr int LDK = kvt_ldk(DIM), LDV = kvt_ldv(DIM), KS = DIM / 16, DB = DIM / 32, BM = 32 * W, RING = 4, NS = KVT_PLACES;
     extern __shared__ __attribute__((aligned(16))) char kvt_lds_[];
     char* Ks = kvt_lds_; char* Vs = Ks + 2 * KT * LDK;
     uint32_t* Sl = (uint32_t*)(Vs + 2 * KT * LDV);            // [NS][KT] where the keys of tile c lie, in units of 16 bytes, at c modulo NS
@@ -56,10 +56,10 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
         return ((uint32_t)table[n] * a.p.page.d + in) * a.p.row16;
     };
     // What depends on nothing is asked for first: the pages of the first eight tiles' keys, the queries, the drafts' parents.
-    uint32_t page[NS * KT / 256], in[NS * KT / 256];
+    uint32_t page[NS * KT / NT], in[NS * KT / NT];
     if (c0 < c1)
 #pragma unroll
-        for (int i = 0; i < NS * KT / 256; i++) page[i] = (uint32_t)table[page_of(min(c0 + 4 * i + (tid >> 6), c1 - 1), lane, in[i])];
+        for (int i = 0; i < NS * KT / NT; i++) page[i] = (uint32_t)table[page_of(min(c0 + W * i + (tid >> 6), c1 - 1), lane, in[i])];
     u32x4 qf[NP][KS];
     const int r = min(rw + col, rows - 1), tk = (int)kv_div((uint32_t)r, a.G);
     {
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     u32x4 kn[PT], vn[PT]; uint32_t ksn[PT], vsn[PT], off[PT], coming[PT];
     const uint8_t* kb = a.p.k + (size_t)it.kvh * a.p.head_bytes; const uint8_t* vb = a.p.v + (size_t)it.kvh * a.p.head_bytes;
     const uint8_t* ksb = a.p.ks + it.kvh * a.p.shead_bytes; const uint8_t* vsb = a.p.vs + it.kvh * a.p.shead_bytes;
-    auto chunk = [&](int j, int& row, int& dc) { const int ch = tid + 256 * j; row = ch / CPR; dc = ch - row * CPR; return NCH % 256 == 0 || ch < NCH; };
+    auto chunk = [&](int j, int& row, int& dc) { const int ch = tid + NT * j; row = ch / CPR; dc = ch - row * CPR; return NCH % NT == 0 || ch < NCH; };
     auto request = [&](const uint8_t* base, const uint8_t* sbase, u32x4* w, uint32_t* s, uint32_t at, int j) {
         int row, dc;
         if (!chunk(j, row, dc)) return;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     if (c0 < c1) {
         if (tid == 0) *Odd = 0;
 #pragma unroll
-        for (int i = 0; i < NS * KT / 256; i++) Sl[((c0 + 4 * i + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[i] * a.p.page.d + in[i]) * a.p.row16;
+        for (int i = 0; i < NS * KT / NT; i++) Sl[((c0 + W * i + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[i] * a.p.page.d + in[i]) * a.p.row16;
         __syncthreads();
         places(c0, off); places(c0 + 1, coming);
         u32x4 k2[PT]; uint32_t ks2[PT];
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
             __syncthreads();
             // the places of tiles c + 8 .. c + 11: their pages are asked for, and a tile later they take the place of tiles whose keys have all been asked for
             const int turn = (c - c0) & 3;
-            if (turn == 0) page[0] = (uint32_t)table[page_of(min(c + NS + (tid >> 6), c1 - 1), lane, in[0])];
+            if (turn == 0 && wave < 4) page[0] = (uint32_t)table[page_of(min(c + NS + (tid >> 6), c1 - 1), lane, in[0])];
             scores(c, 1, sb, sa, c, 0, yes());
             if (c < wf || c >= wt) mask(c, 1, sb);
             settle(sa);
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
             settle(sb);
             places(c + 3, coming);
             sums(c, 1, c + 1, 1, yes());
-            if (turn == 1) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[0] * a.p.page.d + in[0]) * a.p.row16;
+            if (turn == 1 && wave < 4) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[0] * a.p.page.d + in[0]) * a.p.row16;
         }
         __syncthreads();
         if (*Odd) {                                           // the values that became 0 above: every row takes those that it sees
@@ -377,19 +377,23 @@ __global__ void __launch_bounds__(256, kv_tile_waves(DIM)) kr_kv_tile_kernel(con
     }
 }
 
-template <int DIM, int FMT, bool HQ> static int kvt_launch(const KvAttnArgs& a, hipStream_t st) {
+template <int DIM, int FMT, bool HQ, int W> static int kvt_launch(const KvAttnArgs& a, hipStream_t st) {
     constexpr size_t lds = kvt_lds(DIM);
-    if (lds > 65536 && kr_lds_optin((const void*)kr_kv_tile_kernel<DIM, FMT, HQ>, lds)) return 1;
-    hipLaunchKernelGGL((kr_kv_tile_kernel<DIM, FMT, HQ>), dim3(a.items), dim3(256), lds, st, a);
+    if (lds > 65536 && kr_lds_optin((const void*)kr_kv_tile_kernel<DIM, FMT, HQ, W>, lds)) return 1;
+    hipLaunchKernelGGL((kr_kv_tile_kernel<DIM, FMT, HQ, W>), dim3(a.items), dim3(64 * W), lds, st, a);
     return 0;
 }
-template <int FMT> static int kvt_dim(const KvAttnArgs& a, int dim, int half, hipStream_t st) {
+template <int DIM, int FMT> static int kvt_waves(const KvAttnArgs& a, int half, int waves, hipStream_t st) {
+    if constexpr (DIM == 96 || DIM == 128) if (waves == 8) return half ? kvt_launch<DIM, FMT, true, 8>(a, st) : kvt_launch<DIM, FMT, false, 8>(a, st);
+    return waves != 4 ? 1 : half ? kvt_launch<DIM, FMT, true, 4>(a, st) : kvt_launch<DIM, FMT, false, 4>(a, st);
+}
+template <int FMT> static int kvt_dim(const KvAttnArgs& a, int dim, int half, int waves, hipStream_t st) {
     switch (dim) {
-        case 64: return half ? kvt_launch<64, FMT, true>(a, st) : kvt_launch<64, FMT, false>(a, st);
-        case 96: return half ? kvt_launch<96, FMT, true>(a, st) : kvt_launch<96, FMT, false>(a, st);
-        case 128: return half ? kvt_launch<128, FMT, true>(a, st) : kvt_launch<128, FMT, false>(a, st);
-        case 192: return half ? kvt_launch<192, FMT, true>(a, st) : kvt_launch<192, FMT, false>(a, st);
-        case 256: return half ? kvt_launch<256, FMT, true>(a, st) : kvt_launch<256, FMT, false>(a, st);
+        case 64: return kvt_waves<64, FMT>(a, half, waves, st);
+        case 96: return kvt_waves<96, FMT>(a, half, waves, st);
+        case 128: return kvt_waves<128, FMT>(a, half, waves, st);
+        case 192: return kvt_waves<192, FMT>(a, half, waves, st);
+        case 256: return kvt_waves<256, FMT>(a, half, waves, st);
     }
     return 1;
 }
