@@ -254,9 +254,9 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
         }
         l += hs;
     };
-    // The product with half tile b's values, while, in the second half, the coming tiles go to LDS, keys of tile c + 2 where tile c's were, values of c + 1,
-    // and those after them are asked for (behind the last tile: some tile's again).
-    auto sums = [&](int c, int b, int kc, int kb_, auto COMMIT) {
+    // The product with half tile b's values, while the coming tiles go to LDS and those after them are asked for (behind the last tile: some tile's again): keys of tile c + 2 where tile
+    // c's were in the first half, values of tile c + 1 in the second.
+    auto sums = [&](int c, int b, int kc, int kb_) {
         const char* vl = values_at(c, b); const char* kl = keys_at(kc, kb_);
         constexpr int STEPS = 2 * DB;
 #pragma unroll
@@ -265,12 +265,10 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
             for (int p = NP - 1; p >= 0; p--) o[i >> 1] = kvt_mfma<HM>(vr[i % RING], pf[p][i & 1], o[i >> 1]);
             if (i + RING < STEPS) vr[i % RING] = value(vl, (i + RING) >> 1, (i + RING) & 1);
             else kr[i + RING - STEPS] = key(kl, i + RING - STEPS);
-            if constexpr (COMMIT) {
 #pragma unroll
-                for (int j = 2 * PT * i / STEPS; j < 2 * PT * (i + 1) / STEPS; j++) {
-                    if (j < PT) { commit(Ks + (c & 1) * KT * LDK, LDK, kn, ksn, j); request(kb, ksb, kn, ksn, coming[j], j); }
-                    else { commit(Vs + ((c + 1) & 1) * KT * LDV, LDV, vn, vsn, j - PT); request(vb, vsb, vn, vsn, off[j - PT], j - PT); off[j - PT] = coming[j - PT]; }
-                }
+            for (int j = PT * i / STEPS; j < PT * (i + 1) / STEPS; j++) {
+                if (b == 0) { commit(Ks + (c & 1) * KT * LDK, LDK, kn, ksn, j); request(kb, ksb, kn, ksn, coming[j], j); }
+                else { commit(Vs + ((c + 1) & 1) * KT * LDV, LDV, vn, vsn, j); request(vb, vsb, vn, vsn, off[j], j); off[j] = coming[j]; }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -310,15 +308,16 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
             if (turn == 0 && wave < 4) page[0] = (uint32_t)table[page_of(min(c + NS + (tid >> 6), c1 - 1), lane, in[0])];
             scores(c, 1, sb, sa, c, 0, yes());
             if (c < wf || c >= wt) mask(c, 1, sb);
+            places(c + 3, coming);                            // not used where there is no such tile
             settle(sa);
-            sums(c, 0, c + 1, 0, no());
+            __syncthreads();                                  // every wave has multiplied tile c's keys: the next ones may take their place
+            sums(c, 0, c + 1, 0);
             scores(c + 1, 0, sa, sb, c, 1, yes());            // behind the last tile: of no use, and harmless
             const bool more = c + 1 < c1;
             if (more && (c + 1 < wf || c + 1 >= wt)) mask(c + 1, 0, sa);
             if (more && (c + 1 < gf || c + 1 >= gt)) look();
             settle(sb);
-            places(c + 3, coming);
-            sums(c, 1, c + 1, 1, yes());
+            sums(c, 1, c + 1, 1);
             if (turn == 1 && wave < 4) Sl[((c - 1 + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[0] * a.p.page.d + in[0]) * a.p.row16;
         }
         __syncthreads();
