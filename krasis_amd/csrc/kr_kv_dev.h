@@ -55,8 +55,7 @@ __device__ __forceinline__ uint64_t kv_ancestors(const int* parents, int n, int 
     int par = lane < n ? parents[lane] : -1;
     if (par >= lane || par < 0) par = -1;
     uint64_t seen = 1ull << lane;
-#pragma unroll
-    for (int r = 0; r < 6; r++) {
+    for (int r = 0; r < 6 && __any(par >= 0); r++) {
         const int from = par < 0 ? lane : par;
         const uint32_t lo = __shfl((uint32_t)seen, from), hi = __shfl((uint32_t)(seen >> 32), from);
         const int up = __shfl(par, from);

@@ -38,44 +38,56 @@ template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_ke
             *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};
         }
     } else {
-        __shared__ float wl[KV_MAX_SHARES]; __shared__ float red[8]; __shared__ float4 sums[256];
+        __shared__ float wl[KV_MAX_SHARES], dl[KV_MAX_SHARES]; __shared__ float red[8]; __shared__ float4 sums[256];
         const int r = it.split, rr = it.rt * bm + r;
         if (rr >= rows) return;
-        float top = -INFINITY, den = 0.0f;
-        for (int s = tid; s < it.nsplit; s += 256) { const float ms = stats[((size_t)(first + s * step) * bm + r) * 2]; wl[s] = ms; top = fmaxf(top, ms); }
+        const int groups = 256 / quads, g = tid / quads, d = tid % quads * 4;
+        const float* wp = a.ws + ((size_t)first * bm + r) * dim + d; const size_t next = (size_t)step * bm * dim;
+        float4 x[4];                                          // a thread's first shares, on their way while the weights are found
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        for (int u = 0; u < 4; u++) x[u] = *reinterpret_cast<const float4*>(wp + (size_t)min(g + u * groups, it.nsplit - 1) * next);
+        float top = -INFINITY, den = 0.0f;
+        for (int s = tid; s < it.nsplit; s += 256) {
+            const float2 st = *reinterpret_cast<const float2*>(stats + ((size_t)(first + s * step) * bm + r) * 2);
+            wl[s] = st.x; dl[s] = st.y; top = fmaxf(top, st.x);
+        }
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
         if ((tid & 63) == 0) red[tid >> 6] = top;
         __syncthreads();
         top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float base = top == -INFINITY ? 0.0f : top;
         for (int s = tid; s < it.nsplit; s += 256) {
-            const float ms = wl[s], ls = stats[((size_t)(first + s * step) * bm + r) * 2 + 1];
-            const bool none = ms == -INFINITY && ls == 0.0f;
-            const float f = none ? -1.0f : __builtin_amdgcn_exp2f(ms - base);      // -1: a share without keys of this row
+            const bool none = wl[s] == -INFINITY && dl[s] == 0.0f;
+            const float f = none ? -1.0f : __builtin_amdgcn_exp2f(wl[s] - base);      // -1: a share without keys of this row
+            if (!none) den += dl[s] * f;
             wl[s] = f;
-            if (!none) den += ls * f;
         }
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) den += __shfl_xor(den, d);
+        for (int k = 1; k < 64; k <<= 1) den += __shfl_xor(den, k);
         if ((tid & 63) == 0) red[4 + (tid >> 6)] = den;
         __syncthreads();
         den = red[4] + red[5] + red[6] + red[7];
-        const int groups = 256 / quads, g = tid / quads, d = tid % quads * 4;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (g < groups) {
-            const float* wp = a.ws + ((size_t)first * bm + r) * dim + d;
-#pragma unroll 4
-            for (int s = g; s < it.nsplit; s += groups) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int s = g + u * groups;
+                if (s >= it.nsplit || wl[s] == -1.0f) continue;
                 const float f = wl[s];
-                const float4 x = *reinterpret_cast<const float4*>(wp + (size_t)s * step * bm * dim);
-                if (f != -1.0f) { o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f; }
+                o.x += x[u].x * f; o.y += x[u].y * f; o.z += x[u].z * f; o.w += x[u].w * f;
+            }
+#pragma unroll 4
+            for (int s = g + 4 * groups; s < it.nsplit; s += groups) {
+                const float f = wl[s];
+                const float4 y = *reinterpret_cast<const float4*>(wp + (size_t)s * next);
+                if (f != -1.0f) { o.x += y.x * f; o.y += y.y * f; o.z += y.z * f; o.w += y.w * f; }
             }
         }
         sums[tid] = o;
         __syncthreads();
         if (tid >= quads) return;
-        for (int k = 1; k < groups; k++) { const float4 x = sums[k * quads + tid]; o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w; }
+        for (int k = 1; k < groups; k++) { const float4 y = sums[k * quads + tid]; o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w; }
         const float inv = den == 0.0f ? 0.0f : 1.0f / den;
         const int t = (int)kv_div((uint32_t)rr, a.G), h = it.kvh * G + rr - t * G;
         *reinterpret_cast<u32x2*>(a.out + ((size_t)(it.row0 + t) * a.heads + h) * dim + d) = u32x2{kv_pack<H>(o.x * inv, o.y * inv), kv_pack<H>(o.z * inv, o.w * inv)};

@@ -207,7 +207,7 @@ def unpage_into_store(store, seq_state: SequenceKVState, layer_map, kv_max_seq: 
         pair = []
         for t in (a, b):
             keep_bytes = fp8_store and t.dtype == torch.float8_e4m3fn
-            flat = (t.reshape(seq_state.seq_len, -1) if batch is not None else seq_state.unpage(t, None if keep_bytes else torch.float16)).cpu().contiguous()
+            flat = (t.flatten(1) if batch is not None else seq_state.unpage(t, None if keep_bytes else torch.float16)).cpu().contiguous()
             host = flat.view(torch.uint8).numpy() if keep_bytes else flat.view(torch.int16).numpy().view(np.uint16)
             full = np.zeros((kv_max_seq, host.shape[1]), host.dtype)
             full[: host.shape[0]] = host
