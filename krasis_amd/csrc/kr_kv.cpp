@@ -169,7 +169,7 @@ extern "C" int kr_kv_plan(int n_pages, int page_tokens, int batch, const int* le
     try {
         int* row0 = plan + H_SIZE; int* ln = row0 + batch + 1; int* page0 = ln + batch; int* pages = page0 + batch; int* slots = pages + entries;
         std::vector<uint8_t> written((size_t)n_pages, 0);
-        bool own = true;
+        bool own = true;                                      // no slot twice: a page that gets rows twice may still hold them apart
         int r = 0, e = 0; int64_t t0 = 0;
         for (int b = 0; b < batch; b++) {
             row0[b] = r; ln[b] = lens[b]; page0[b] = e;
@@ -189,6 +189,11 @@ extern "C" int kr_kv_plan(int n_pages, int page_tokens, int batch, const int* le
             e += n; t0 += table_lens[b];
         }
         row0[batch] = r;
+        if (!own) {
+            std::vector<int> sorted(slots, slots + r);
+            std::sort(sorted.begin(), sorted.end());
+            own = std::adjacent_find(sorted.begin(), sorted.end()) == sorted.end();
+        }
         for (int i = 0; i < H_SIZE; i++) plan[i] = 0;
         plan[H_BATCH] = batch; plan[H_ROWS] = r; plan[H_ENTRIES] = e; plan[H_PAGE_TOKENS] = page_tokens; plan[H_PAGES] = n_pages; plan[H_OWN] = own;
     } catch (const std::exception& x) { return kr_fail(KR_ERR_STATE, "kr_kv_plan: %s", x.what()); }

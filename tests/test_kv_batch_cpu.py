@@ -172,3 +172,14 @@ def test_workspaces_grow_with_the_shares():
         return size.value
     assert need([short], [1], 16) == 0 and need([long], [1], 16) > 0 and need([long], [40], 16, tree=1) > 0
     assert need([long], [1], 16, window=32) == 0
+
+
+def test_sequences_may_write_to_different_slots_of_a_page():
+    from krasis_amd.kv_cache import plan_of
+    cache = make_cache(2, 64, "mx8", 16, device="cpu")
+    a, b = states(cache, [20, 26])
+    b.pages[1] = a.pages[1]                                         # a's rows at 4 and 5 of the page, b's at 10 and 11
+    assert plan_of(cache, [a, b], [2, 2])[5] == 1
+    assert plan_of(cache, [a, b], [7, 2])[5] == 0                   # a's at 4 to 10
+    a.pages = tuple(a.pages)
+    assert plan_of(cache, [a], [2])[5] == 1

@@ -445,3 +445,34 @@ def test_refusals():
     (s,) = sequences(f, [5])
     with pytest.raises(ValueError, match="another 16-bit type"):
         KVBatch(f, [s], [3]).attend(0, ok)
+
+
+def test_arguments_wider_than_the_librarys_are_refused():
+    from krasis_amd.kv_cache import KVBatch
+    cache = make_cache(2, 64, "mx8", 20)
+    fill(cache, "mx8", 1)
+    (s,) = sequences(cache, [5])
+    b, q = KVBatch(cache, [s], [3]), rows(3, 2, 64, torch.bfloat16, 1)
+    for window, first in ((2 ** 32 + 2, 0), (2, 2 ** 32), (2 ** 31, 0), (2, -1), (-2 ** 32 + 2, 0)):
+        with pytest.raises(ValueError, match="window"):
+            b.attend(0, q, window=window, keep_first=first)
+        with pytest.raises(ValueError, match="window"):
+            b.attend_tree(0, q, [-1, 0, 1], window=window, keep_first=first)
+    assert torch.equal(b.attend(0, q), b.attend(0, q, window=2 ** 31 - 1, keep_first=2 ** 31 - 1))
+
+
+@pytest.mark.parametrize("end", ["commit", "keep"])
+def test_a_batch_ends_on_the_sequences_that_it_was_made_for(end):
+    from krasis_amd.kv_cache import KVBatch
+    cache = make_cache(2, 64, "mx8", 20)
+    a, b = sequences(cache, [5, 7])
+    one, two = KVBatch(cache, [a], [3]), KVBatch(cache, [a, b], [2, 1])      # both write a's places from 5 on
+    one.commit()
+    with pytest.raises(RuntimeError, match="has changed"):
+        two.commit() if end == "commit" else two.keep([[0], [0]])
+    assert (a.seq_len, b.seq_len) == (8, 7)
+    late = KVBatch(cache, [b], [1])
+    b.free()
+    with pytest.raises(RuntimeError, match="has changed"):
+        late.commit() if end == "commit" else late.keep([[0]])
+    assert b.seq_len == 0
