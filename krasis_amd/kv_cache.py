@@ -328,8 +328,8 @@ class KVBatch:
         if dtype not in _ROWS:
             raise ValueError(f"rows are read as bfloat16 or float16, not {dtype}")
         h, d = self.cache.num_kv_heads, self.cache.gqa_head_dim
-        k = torch.empty((self.rows, h, d), dtype=dtype, device=self.device)
-        v = torch.empty((self.rows, h, d), dtype=dtype, device=self.device)
+        # one allocation, its strides given: a call on few rows takes the time of its host code
+        k, v = torch.empty_strided((2, self.rows, h, d), (self.rows * h * d, h * d, d, 1), dtype=dtype, device=self.device).unbind(0)
         self._call(self._lib.kr_kv_read, self._layer(layer), *self._plan, k.data_ptr(), v.data_ptr(), _Strides(h * d, d, h * d, d), _ROWS[dtype])
         return k, v
 
@@ -377,7 +377,7 @@ class KVBatch:
         if not 0 <= window <= _INT_MAX or not 0 <= keep_first <= _INT_MAX:
             raise ValueError(f"window {window}, keep_first {keep_first}: 0 to {_INT_MAX}")
         if out is None:
-            out = torch.empty((self.rows, heads, d), dtype=q.dtype, device=self.device)
+            out = torch.empty_strided((self.rows, heads, d), (heads * d, d, 1), dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"out: contiguous {q.dtype} {tuple(q.shape)} on {q.device}, aligned to 16 bytes")
         pages, key = self._layer(layer), (heads, q.dtype, window, keep_first, parents is not None)
@@ -386,7 +386,7 @@ class KVBatch:
             size = ctypes.c_size_t()
             _lib.check(self._lib.kr_kv_attend_workspace(pages, self._plan[0], heads, _ROWS[q.dtype], window, keep_first, int(parents is not None), ctypes.byref(size)))
             self._need[key] = need = size.value
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None      # of this call alone: two streams, or two graphs, never share one
+        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=self.device) if need else None      # of this call alone: two streams, or two graphs, never share one
         self._call(self._lib.kr_kv_attend, pages, *self._plan, q.data_ptr(), qt, qh, out.data_ptr(), _ROWS[q.dtype], heads, d ** -0.5 if scale is None else scale,
                    window, keep_first, None if parents is None else parents.data_ptr(), None if ws is None else ws.data_ptr(), need)
         return out
