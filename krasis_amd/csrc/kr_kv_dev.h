@@ -140,3 +140,16 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& i
     r.tiles = r.kept + (r.hi - r.start + kt - 1) / kt;
     return r;
 }
+
+// the keys [first, first + 32) that a row sees, of those before `end`: bit k for key first + k.  pos: the row's position; seen: its drafts (those outside its window left out)
+__device__ __forceinline__ uint32_t kv_below(int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1; }
+__device__ __forceinline__ uint32_t kv_visible(const KvAttnArgs& a, const KvRange& rg, int first, int end, int pos, uint64_t seen) {
+    const int before = rg.before - first;
+    uint32_t ok = a.parents ? kv_below(before) : kv_below(pos + 1 - first);
+    if (a.window > 0) ok &= ~kv_below(pos - a.window + 1 - first) | kv_below(a.first - first);
+    if (a.parents) {
+        const uint32_t up = before >= 32 ? 0u : (uint32_t)(seen << (before & 31)), down = before <= -64 ? 0u : (uint32_t)(seen >> (-before & 63));
+        ok |= before >= 0 ? up : down;
+    }
+    return ok & kv_below(end - first);
+}

@@ -70,12 +70,17 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
     auto scale_of = [&](uint32_t byte) { return kv_scale((byte & a.p.scale_and) | a.p.scale_or); };
 
     // the row's position, and which drafts it sees
-    int pos = rg.before + t; uint64_t seen = 0; int depth = 0;
+    int pos = rg.before + t; uint64_t seen = 0;
     if (!ONE && a.parents) {
         const uint64_t all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
-        depth = __popcll(all) - 1;                            // of draft `lane`
+        const int depth = __popcll(all) - 1;                  // of draft `lane`
         seen = (uint64_t)__shfl((uint32_t)(all >> 32), t) << 32 | __shfl((uint32_t)all, t);
         pos = rg.before + __shfl(depth, t);
+        if (a.window > 0 && it.cnt > a.window)                // ancestors outside the window
+            for (int n = 0; n < it.cnt; n++) {
+                const int d = __shfl(depth, n);
+                if (pos - rg.before - d >= a.window && rg.before + d >= a.first) seen &= ~(1ull << n);
+            }
     }
     // the query row: dims q DIM / 4 + 8 i
     u32x4 qf[NP][U];
@@ -167,19 +172,11 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
         __builtin_amdgcn_sched_barrier(0);
         // scores of keys that a row does not see, where the tile has some
         if (j0 + 32 > end || j0 + 31 > rg.before - (!ONE && a.parents ? 1 : 0) || (a.window > 0 && rg.before + it.cnt - 1 - j0 >= a.window && j0 + 32 > a.first)) {
+            const uint32_t ok = kv_visible(a, rg, j0 + 4 * q, end, pos, seen);
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = j0 + b * 16 + 4 * q + i;
-                    int at = key; bool ok = key < end;
-                    if (!ONE && a.parents) {
-                        const int n = key - rg.before, d = __shfl(depth, n & 63);
-                        if (n >= 0) { at = rg.before + d; ok = ok && (seen >> (n & 63) & 1); }
-                    } else ok = ok && key <= pos;
-                    if (a.window > 0) ok = ok && (pos - at < a.window || at < a.first);
-                    if (!ok) st[b][i] = -INFINITY;
-                }
+                for (int i = 0; i < 4; i++) if (!(ok >> (16 * b + i) & 1)) st[b][i] = -INFINITY;
         }
         // Weights from a reference, exp2(s - m): a row's first maximum in this wave, which moves, with what was summed so far, when a lane's sum gets out of the numbers' range (f16 ends at
         // 2^16, bf16 and 32 bits are far from their end), and until the row has seen its first key.  NaN scores move nothing and are in the sums.

@@ -144,18 +144,21 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
         for (int j = 0; j < PT; j++) {
             int row, dc;
             if (!chunk(j, row, dc)) break;
+            // all ones in a field, and one more: a carry into the sign's place of its number
             if constexpr (FMT == 0) {
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int u = 0; u < 32; u += 16) if ((vn[j][e] >> u & EXP) == EXP) { vn[j][e] &= ~(0xFFFFu << u); odd = true; }
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t bad = ((vn[j][e] & EXP * 0x10001u) + (EXP & -EXP) * 0x10001u) & 0x80008000u;
+                    vn[j][e] &= ~((bad << 1) - (bad >> 15)); odd = odd || bad;
+                }
             } else {
                 if (((vsn[j] & a.p.scale_and) | a.p.scale_or) == 255u) { vn[j] = u32x4{0, 0, 0, 0}; vsn[j] = 127; odd = true; }
                 if constexpr (FMT == 1)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-#pragma unroll
-                        for (int u = 0; u < 32; u += 8) if ((vn[j][e] >> u & 0x7Fu) == 0x7Fu) { vn[j][e] &= ~(0xFFu << u); odd = true; }
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t bad = ((vn[j][e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                        vn[j][e] &= ~((bad << 1) - (bad >> 7)); odd = odd || bad;
+                    }
             }
         }
         if (odd) *Odd = 1;
@@ -220,18 +223,13 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto mask = [&](int c, int b, kv_f16& s) {          // scores of keys that a row does not see
-        const int j0 = first_key(c), end = c < rg.kept ? min(a.first, rg.hi) : rg.hi;
+    // Scores of keys that a row does not see: 32 keys from the lane's first one on are a word, put together without a branch.  Key by key, with the drafts' depths from LDS, a half tile
+    // took 3 us where this takes a tenth.
+    auto mask = [&](int c, int b, kv_f16& s) {
+        const int first = first_key(c) + 32 * b + 4 * h;
+        const uint32_t ok = kv_visible(a, rg, first, c < rg.kept ? min(a.first, rg.hi) : rg.hi, pos, seen);
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int key = j0 + 32 * b + (i & 3) + 8 * (i >> 2) + 4 * h, n = key - rg.before;
-            const int at = a.parents && n >= 0 ? rg.before + Dp[n & (KV_MAX_TREE - 1)] : key;
-            bool ok = key < end;
-            if (a.parents) { if (n >= 0) ok = ok && (seen >> (n & 63) & 1); }
-            else ok = ok && key <= pos;
-            if (a.window > 0) ok = ok && (pos - at < a.window || at < a.first);
-            if (!ok) s[i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; i++) if (!(ok >> ((i & 3) + 8 * (i >> 2)) & 1)) s[i] = -INFINITY;
     };
     // The weights stand when no sum of a half tile is out of bounds (f16 ends at 2^16, bf16 and 32 bits are far from their end); else, and until a row has seen its first key, the
     // references move to the maxima, and what was summed so far with them.  NaN scores move nothing and are in the sums.
@@ -279,6 +277,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
 #pragma unroll
         for (int i = 0; i < NS * KT / NT; i++) Sl[((c0 + W * i + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[i] * a.p.page.d + in[i]) * a.p.row16;
         __syncthreads();
+        if (a.parents && a.window > 0 && it.cnt > a.window)   // ancestors outside the window
+            for (int n = 0; n < it.cnt; n++) if (pos - rg.before - Dp[n] >= a.window && rg.before + Dp[n] >= a.first) seen &= ~(1ull << n);
         places(c0, off); places(c0 + 1, coming);
         u32x4 k2[PT]; uint32_t ks2[PT];
 #pragma unroll
