@@ -277,8 +277,16 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
 #pragma unroll
         for (int i = 0; i < NS * KT / NT; i++) Sl[((c0 + W * i + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[i] * a.p.page.d + in[i]) * a.p.row16;
         __syncthreads();
-        if (a.parents && a.window > 0 && it.cnt > a.window)   // ancestors outside the window
-            for (int n = 0; n < it.cnt; n++) if (pos - rg.before - Dp[n] >= a.window && rg.before + Dp[n] >= a.first) seen &= ~(1ull << n);
+        if (a.parents && a.window > 0 && it.cnt > a.window) {  // ancestors outside the window, eight drafts at a time
+            const int last = pos - rg.before - a.window, least = a.first - rg.before;
+            for (int n = 0; n < it.cnt; n += 8) {
+                int d[8]; uint32_t out = 0;
+                *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(Dp + n); *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(Dp + n + 4);
+#pragma unroll
+                for (int u = 0; u < 8; u++) out |= d[u] <= last && d[u] >= least ? 1u << u : 0u;
+                seen &= ~((uint64_t)out << n);
+            }
+        }
         places(c0, off); places(c0 + 1, coming);
         u32x4 k2[PT]; uint32_t ks2[PT];
 #pragma unroll
