@@ -213,7 +213,11 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
 #pragma unroll
         for (int i = 0; i < KS; i++) {
 #pragma unroll
-            for (int p = NP - 1; p >= 0; p--) n = kvt_mfma<HM>(kr[i % RING], qf[p][i], n);
+            for (int p = NP - 1; p >= 0; p--) {
+                // queries that do not fit into the first 256 registers stay in the accumulation registers, which a product reads in place
+                if constexpr (DIM > 128) asm volatile("" : "+a"(qf[p][i]));
+                n = kvt_mfma<HM>(kr[i % RING], qf[p][i], n);
+            }
             if (i + RING < KS) kr[i % RING] = key(kl, i + RING);
             else vr[i + RING - KS] = value(vl, (i + RING - KS) >> 1, (i + RING - KS) & 1);
             if constexpr (WEIGH) {
