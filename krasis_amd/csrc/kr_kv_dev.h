@@ -50,9 +50,8 @@ template <bool H> __device__ __forceinline__ float kv_sum2(uint32_t w, float c) 
 __device__ __forceinline__ uint32_t kv_rest(float a, float b, uint32_t w) { return kv_pack<false>(a - kv_lo(w), b - kv_hi(w)); }
 
 // ancestors of the drafts of one sequence, lane i: bit j set when draft j is draft i or an ancestor.  Parents are doubled up: after k rounds a lane knows 2^k ancestors.
-// A parent that is no earlier draft counts as none.
-__device__ __forceinline__ uint64_t kv_ancestors(const int* parents, int n, int lane) {
-    int par = lane < n ? parents[lane] : -1;
+// par: the parent of draft `lane`; one that is no earlier draft counts as none.
+__device__ __forceinline__ uint64_t kv_ancestors(int par, int lane) {
     if (par >= lane || par < 0) par = -1;
     uint64_t seen = 1ull << lane;
     for (int r = 0; r < 6 && __any(par >= 0); r++) {

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
     // the row's position, and which drafts it sees
     int pos = rg.before + t; uint64_t seen = 0;
     if (!ONE && a.parents) {
-        const uint64_t all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
+        const uint64_t all = kv_ancestors(lane < it.cnt ? a.parents[it.row0 + lane] : -1, lane);
         const int depth = __popcll(all) - 1;                  // of draft `lane`
         seen = (uint64_t)__shfl((uint32_t)(all >> 32), t) << 32 | __shfl((uint32_t)all, t);
         pos = rg.before + __shfl(depth, t);

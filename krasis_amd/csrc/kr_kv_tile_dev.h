@@ -70,13 +70,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
 #pragma unroll
         for (int i = 0; i < KS; i++) qf[0][i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
     }
+    const int parent = a.parents && lane < it.cnt ? a.parents[it.row0 + lane] : -1;
     int pos = rg.before + tk; uint64_t seen = 0;
-    if (a.parents) {
-        const uint64_t all = kv_ancestors(a.parents + it.row0, it.cnt, lane);
-        if (tid < KV_MAX_TREE) Dp[tid] = __popcll(all) - 1;
-        seen = (uint64_t)__shfl((uint32_t)(all >> 32), tk) << 32 | __shfl((uint32_t)all, tk);
-        pos = rg.before + __popcll(seen) - 1;
-    }
     auto queries = [&]() {                                    // as they enter the products: the scale's sign, two pieces of f16 where the products are bf16
         const uint32_t sign = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
@@ -284,20 +279,16 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
 #pragma unroll
         for (int i = 0; i < NS * KT / NT; i++) Sl[((c0 + W * i + (tid >> 6)) & (NS - 1)) * KT + lane] = (page[i] * a.p.page.d + in[i]) * a.p.row16;
         __syncthreads();
-        if (a.parents && a.window > 0 && it.cnt > a.window) {  // ancestors outside the window, eight drafts at a time
-            const int last = pos - rg.before - a.window, least = a.first - rg.before;
-            for (int n = 0; n < it.cnt; n += 8) {
-                int d[8]; uint32_t out = 0;
-                *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(Dp + n); *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(Dp + n + 4);
-#pragma unroll
-                for (int u = 0; u < 8; u++) out |= d[u] <= last && d[u] >= least ? 1u << u : 0u;
-                seen &= ~((uint64_t)out << n);
-            }
-        }
         places(c0, off); places(c0 + 1, coming);
         u32x4 k2[PT]; uint32_t ks2[PT];
 #pragma unroll
         for (int j = 0; j < PT; j++) { request(kb, ksb, kn, ksn, off[j], j); request(vb, vsb, vn, vsn, off[j], j); request(kb, ksb, k2, ks2, coming[j], j); }
+        if (a.parents) {
+            const uint64_t all = kv_ancestors(parent, lane);
+            if (tid < KV_MAX_TREE) Dp[tid] = __popcll(all) - 1;
+            seen = (uint64_t)__shfl((uint32_t)(all >> 32), tk) << 32 | __shfl((uint32_t)all, tk);
+            pos = rg.before + __popcll(seen) - 1;
+        }
         queries();
         if (c0 < gf || c0 >= gt) look();
         places(c0 + 2, off);
@@ -309,6 +300,16 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM)) kr_kv
 #pragma unroll
         for (int j = 0; j < PT; j++) commit(Ks + ((c0 + 1) & 1) * KT * LDK, LDK, k2, ks2, j);
         __syncthreads();
+        if (a.parents && a.window > 0 && it.cnt > a.window) {  // ancestors outside the window, eight drafts at a time
+            const int last = pos - rg.before - a.window, least = a.first - rg.before;
+            for (int n = 0; n < it.cnt; n += 8) {
+                int d[8]; uint32_t out = 0;
+                *reinterpret_cast<int4*>(d) = *reinterpret_cast<const int4*>(Dp + n); *reinterpret_cast<int4*>(d + 4) = *reinterpret_cast<const int4*>(Dp + n + 4);
+#pragma unroll
+                for (int u = 0; u < 8; u++) out |= d[u] <= last && d[u] >= least ? 1u << u : 0u;
+                seen &= ~((uint64_t)out << n);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < RING; i++) kr[i] = key(keys_at(c0, 0), i);
         scores(c0, 0, sa, sa, c0, 0, no());
