@@ -8,8 +8,8 @@
 // next half and the coming tiles' conversion go under the product with V; the first fragments of each product are read from LDS under the one before.
 // Weights are measured from a reference, exp2(s - m): a row's first maximum, which moves only when a half tile's sum of weights gets out of the numbers' range (their precision does not
 // depend on it).  No maxima are formed on the way, and O is hardly ever rescaled.
-// Measured: two prompts of 8192 and 3001 tokens (64 / 4 heads of 128, eight bits) 1.02 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 46 % busy at the 1.9 GHz that its
-// power leaves; portions with heads of 256 channels over f16 pages 845 TFLOP/s, one wave a SIMD, 4.7 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
+// Measured: two prompts of 8192 and 3001 tokens (64 / 4 heads of 128, eight bits) 1.03 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 46 % busy at the 1.9 GHz that its
+// power leaves; portions with heads of 256 channels over f16 pages 863 TFLOP/s, one wave a SIMD, 4.7 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
 // tile of 128 channels 1.3 us alone: short sequences are bound by that.
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
