@@ -135,7 +135,7 @@ void parts_of(const Plan& h, int kv_heads, int heads, int dim, int fmt, bool hal
     for (int b = 0; b < h.batch && one; b++) { const int64_t cnt = h.row0[b + 1] - h.row0[b]; one = cnt <= 1 || cnt * G > KV_STEP_BM; }
     p[0].one = one;
     divide(h, kv_heads, G, window, first, tree, 1, kv_step_waves(dim, fmt, half, one), 3, 3, p[0]);
-    divide(h, kv_heads, G, window, first, tree, waves == 8 ? 1 : kv_tile_waves(dim, half && fmt != 0), 1, 6, 4, p[1]);
+    divide(h, kv_heads, G, window, first, tree, waves == 8 ? 1 : kv_tile_waves(dim, fmt, half), 1, 6, 4, p[1]);
 }
 size_t part_bytes(const Part& p, int dim) { return p.split ? (size_t)p.items * p.bm * (dim + 2) * sizeof(float) : 0; }
 

@@ -28,7 +28,7 @@ template <bool H> __device__ __forceinline__ kv_f16 kvt_mfma(u32x4 x, u32x4 y, k
 }
 
 template <int DIM, int FMT, bool HQ, int W>
-__global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, HQ && FMT != 0)) kr_kv_tile_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, HQ)) kr_kv_tile_kernel(const KvAttnArgs a) {
     constexpr bool HM = HQ && FMT == 0;
     constexpr int NP = HQ && !HM ? 2 : 1;                     // bf16 pieces of an f16 query and of its weights
     constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, CPR = DIM * BITS / 128, NCH = KT * CPR, NT = 64 * W, PT = (NCH + NT - 1) / NT, CD = 128 / BITS;      // chunks of 16 bytes, CD channels
