@@ -61,7 +61,10 @@ constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads
 constexpr int KV_TILE_KT = 64;                       // keys of a tile in kr_kv_tile_dev.h; 32 rows a wave
 // Waves that a SIMD holds of the latter, by registers and LDS.  Heads of 64 channels take three where their 168 registers suffice, bf16 queries over eight and four bits: two prompts of 8192
 // and 3001 tokens 405 -> 382 us.  Others would spill: 16-bit pages 390 us with two, 498 with three, f16 queries over eight bits 595 and 690.
-__host__ __device__ constexpr int kv_tile_waves(int dim, int fmt, bool half) { return dim == 64 && fmt != 0 && !half ? 3 : dim <= 128 ? 2 : 1; }
+// Of 128 channels f16 queries over eight bits alone spill with two (four waves a workgroup): 64 sequences' drafts 96 us with one, 122 with two; over four bits 96 and 82, 16-bit pages 82 and 79.
+__host__ __device__ constexpr int kv_tile_waves(int dim, int fmt, bool half) {
+    return dim == 64 && fmt != 0 && !half ? 3 : dim < 128 || (dim == 128 && !(fmt == 1 && half)) ? 2 : 1;
+}
 // waves of a workgroup in kr_kv_step_dev.h, one workgroup a CU: by registers.  half: f16 queries (two pieces over pages that become bf16); one: every sequence has one new token
 __host__ __device__ constexpr int kv_step_waves(int dim, int fmt, bool half, bool one) {
     return !one ? (dim <= 128 ? 8 : 4) : dim == 64 || (dim == 96 && fmt == 0) || (dim == 128 && fmt == 2 && !half) ? 16 : dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8;
