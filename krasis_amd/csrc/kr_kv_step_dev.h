@@ -172,9 +172,11 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
         uint32_t coming = 0;
         if constexpr (MORE) { coming = place(); request_k(coming); }
         __builtin_amdgcn_sched_barrier(0);
-        // scores of keys that a row does not see, where the tile has some
-        if (j0 + 32 > end || j0 + 31 > rg.before - (!ONE && a.parents ? 1 : 0) || (a.window > 0 && rg.before + it.cnt - 1 - j0 >= a.window && j0 + 32 > a.first)) {
-            const uint32_t ok = kv_visible(a, rg, j0 + 4 * q, end, pos, seen);
+        // scores of keys that a row does not see, where the tile has some (the copies that stand for keys no row sees among them); ok: bit 16 b + i for the lane's key i of block b
+        const bool hidden = j0 + 32 > end || j0 + 31 > rg.before - (!ONE && a.parents ? 1 : 0) || (a.window > 0 && rg.before + it.cnt - 1 - j0 >= a.window && j0 + 32 > a.first);
+        uint32_t ok = 0xFFFFFFFFu;
+        if (hidden) {
+            ok = kv_visible(a, rg, j0 + 4 * q, end, pos, seen);
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -211,11 +213,21 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
         }
         l += hs;
         constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;
-        // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys.
-        const bool look = !ONE && it.cnt > 1;
-        uint32_t vis[4];                                      // ones where the row sees the key, as a fragment
+        // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys: what they do not see becomes 0.
+        // Else such values are looked for (in tiles that all rows see entirely, too: a weight may be too small for the numbers).
+        const bool look = !ONE && (hidden || it.cnt > 1);
+        if constexpr (ONE) if (hidden) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) vis[e] = (st[e >> 1][2 * (e & 1)] == -INFINITY ? 0u : UNIT) | (st[e >> 1][2 * (e & 1) + 1] == -INFINITY ? 0u : UNIT << 16);
+            for (int i = 0; i < 8; i++)
+                if (!(ok >> ((i >> 2) * 16 + (i & 3)) & 1)) {
+#pragma unroll
+                    for (int g = 0; g < GROUPS; g++) {
+#pragma unroll
+                        for (int x = 0; x < VW; x++) vn[i][g][x] = 0;
+                        vsn[i][g] = 127;
+                    }
+                }
+        }
 #pragma unroll
         for (int g = 0; g < GROUPS; g++)
 #pragma unroll
@@ -236,7 +248,9 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
 #pragma unroll
                     for (int e = 0; e < 4; e++) vf[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], u ? 0x07060302u : 0x05040100u);
                     if (odd) {                                // such values apart: whether a row sees one, by kind
-                        const u32x4 see = {vis[0], vis[1], vis[2], vis[3]};
+                        u32x4 see;                            // ones where the row sees the key, as a fragment
+#pragma unroll
+                        for (int e = 0; e < 4; e++) see[e] = (ok >> ((e >> 1) * 16 + 2 * (e & 1)) & 1 ? UNIT : 0u) | (ok >> ((e >> 1) * 16 + 2 * (e & 1) + 1) & 1 ? UNIT << 16 : 0u);
                         u32x4 keep = vf;
 #pragma unroll
                         for (int k = 0; k < 3; k++) {

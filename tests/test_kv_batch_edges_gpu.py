@@ -1,0 +1,96 @@
+"""Operators over a caller's paged cache where numbers are hard: infinities, weights far below another, values near the end of the numbers, shares that are joined; the definition is
+tests/kv_reference.py."""
+import math
+
+import pytest
+import torch
+
+from tests.kv_reference import DTYPES, attend, make_cache, stored_rows, tolerance, visible
+from tests.test_kv_batch_gpu import fill, rows, sequences, stored_poison
+
+pytestmark = pytest.mark.gpu
+
+
+def agrees(got, q, cache, fmt, states, counts, weight, scale=None, window=0, first=0, trees=None, few=None):
+    """every row against the definition; a result that is not finite has to be that very one.  weight: by how much of itself a weight may be off; few: what f16 weights
+    that are subnormal numbers may come to, where that is less than every key's.  Returns the definition's results."""
+    heads, dim = q.shape[1], q.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    r, outs = 0, []
+    for i, (s, n) in enumerate(zip(states, counts)):
+        k, v = stored_rows(cache, s, fmt)
+        see = visible(s.seq_len - n, n, window, first, None if trees is None else trees[i])
+        out, mean, size = attend(q[r:r + n].double(), k, v, see, scale)
+        if not k.isfinite().all():                                  # how large scores are, of keys that are numbers
+            size = attend(q[r:r + n].double(), k.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), v.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), see, scale)[2]
+        tol = tolerance(out, mean, size, dim, s.seq_len, q.dtype, weight)
+        if fmt == "f16":                                            # subnormal weights are off by 2^-25; the row's largest weighs 2^8 or more
+            tol = tol + (s.seq_len * 2.0 ** -33 * v[v.isfinite()].abs().max() if few is None else few)
+        x = got[r:r + n].double()
+        whole = out.isfinite()
+        assert torch.equal(x.isfinite(), whole), (i, n, s.seq_len, (x.isfinite() != whole).nonzero()[:4].tolist())
+        assert torch.equal(x[~whole].nan_to_num(nan=7.0, posinf=1.0, neginf=-1.0), out[~whole].nan_to_num(nan=7.0, posinf=1.0, neginf=-1.0)), (i, n, s.seq_len)
+        bad = (x - out).abs()[whole] > tol[whole]
+        assert not bad.any(), (i, n, s.seq_len, int(bad.sum()), float(((x - out).abs()[whole] / tol[whole]).max()))
+        outs.append(out); r += n
+    assert r == got.shape[0]
+    return torch.cat(outs)
+
+
+def batch_of(cache, lens, counts, seed=0):
+    from krasis_amd.kv_cache import KVBatch
+    states = sequences(cache, [n - c for n, c in zip(lens, counts)], seed)
+    batch = KVBatch(cache, states, counts)
+    for s, c in zip(states, counts):
+        s.advance(c)
+    return batch, states
+
+
+def pages_for(lens, page):
+    return sum(-(-n // page) for n in lens) + 2
+
+
+# ---------------------------------------------------------------------------------------------------------------- infinities
+SPLIT = [6001, 9005]
+
+
+@pytest.mark.parametrize("window,first", [(0, 0), (20, 0), (20, 4), (50, 70)])
+@pytest.mark.parametrize("lens,counts", [([1, 5, 33, 97, 160], [1, 1, 1, 1, 1]), ([1, 5, 33, 97, 161], [1, 1, 1, 2, 1]), ([70, 130, 41], [40, 64, 41]), (SPLIT, [1, 1]), (SPLIT, [2, 1]), (SPLIT, [40, 33])])
+@pytest.mark.parametrize("fmt", ["bf16", "f16"])
+def test_infinite_values_reach_the_rows_that_see_them_as_they_are(fmt, lens, counts, window, first):
+    """Channels apart for each: the last key's, the window's first key's and the first key's values are infinite, one before all windows, one a NaN, and one channel has both signs."""
+    cache = make_cache(2, 64, fmt, pages_for(lens, 16))
+    fill(cache, fmt, 1)
+    batch, states = batch_of(cache, lens, counts)
+    stored_poison(cache, fmt, states)
+    for s, c in zip(states, counts):
+        n = s.seq_len
+        for pos, channel, bad in ((n - 1, 3, math.inf), (max(0, n - 20), 9, -math.inf), (max(0, n - c), 12, -math.inf), (0, 40, math.inf), (n // 2, 20, math.nan), (n // 3, 21, -math.inf),
+                                  (n - 1, 50, -math.inf), (0, 50, math.inf), (min(n - 1, 31), 33, math.inf), (min(n - 1, 64), 34, -math.inf)):
+            cache.v_cache[0, s.pages[pos // 16], pos % 16, 1, channel] = bad
+    q = rows(sum(counts), 6, 64, DTYPES[fmt], 3)
+    got = batch.attend(0, q, window=window, keep_first=first)
+    if not window:
+        assert (max(batch._need.values()) > 0) == (lens is SPLIT)
+    out = agrees(got, q, cache, fmt, states, counts, 2.0 ** -8 if fmt == "bf16" else 2.0 ** -11, window=window, first=first)
+    assert bool((out == math.inf).any()) and bool((out == -math.inf).any()) and bool(out.isfinite().any())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mx8"])
+def test_infinite_keys_draw_everything_or_nothing(fmt):
+    """A key whose products are all -infinity has no weight; one of +infinity leaves no number.  Over pages of eight bits a block that held one reads as NaN."""
+    lens, counts = [33, 90, 200], [1, 2, 40]
+    cache = make_cache(2, 64, fmt, pages_for(lens, 16))
+    fill(cache, fmt, 2)
+    batch, states = batch_of(cache, lens, counts)
+    stored_poison(cache, fmt, states)
+    q = rows(sum(counts), 4, 64, torch.bfloat16, 3).abs()
+    for s in states:
+        at = (0, s.pages[0], 7, 1)
+        if fmt == "bf16":
+            cache.k_cache[at][5] = -math.inf
+        else:
+            cache.k_scale[at][0] = 255
+    got = batch.attend(0, q)
+    out = agrees(got, q, cache, fmt, states, counts, 2.0 ** -8)
+    assert bool(out[:, :2].isfinite().all()) and bool(out[:, 2:].isnan().all() if fmt == "mx8" else out[:, 2:].isfinite().all())
