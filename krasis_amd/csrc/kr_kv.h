@@ -41,7 +41,7 @@ struct KvAttnArgs {
     int min_rows, max_rows;            // the sequences of this launch: those whose new rows times G lie in between
     KvDiv tps;                         // key tiles a workgroup takes at most
     int items, whole, one;                    // whole: items / (8 kv_heads) * (8 kv_heads); one: no sequence of this launch has more than one new token, and there are no trees
-    float* ws;                         // partial results of sequences that are split: [item][KV_BM rows][dim] sums, then [item][rows][2] maximum and denominator
+    float* ws;                         // partial results of sequences that are split: [item][rows][dim] sums, then [item][rows][2] reference (kr_kv_dev.h) and denominator
 };
 
 int kr_launch_kv_write(const KvRowsArgs& a, hipStream_t st);

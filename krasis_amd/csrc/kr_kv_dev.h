@@ -140,6 +140,21 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& i
     return r;
 }
 
+// ---- references of the softmax: weights are exp2(score - m), and m, -infinity until the row has seen a key, is no more than a measure that sums and weights share.  It stands while a lane's
+// sum of weights (of 8 keys or 16) lies in bounds and moves, with what was summed so far, when it does not.
+// f16 weights (HM) are subnormal numbers below 2^-14 and end at 2^16.  The reference is 2^-8 of the largest weight it was taken from, moves up when a sum passes 2^15, and down again when it
+// falls under 2^-6: a key may draw nearly all attention and be worth nothing, and the many far under it are the result.  So the largest weight of a tile's keys is 2^-10 at least, the others are
+// off by 2^-25 at most.  It stays within 2^60 of what was summed, where 32-bit sums of 16-bit numbers have their end far away.
+// bf16 weights have the range of 32 bits, their sums are of no concern up to 2^30.
+template <bool HM> __device__ __forceinline__ bool kv_out_of_bounds(float sum, float most) { return sum > most || (HM && sum < 0.015625f); }
+// most: -1 until the row has seen a key
+template <bool HM> __device__ __forceinline__ float kv_most(float m) { return m == -INFINITY ? -1.0f : HM ? 32768.0f : 1073741824.0f; }
+// the reference after keys whose largest score is t; sum: all of the row's weights so far
+template <bool HM> __device__ __forceinline__ float kv_reference(float m, float t, float sum) {
+    if constexpr (!HM) return fmaxf(m, t);
+    else return t != -INFINITY && (t > m + 8.0f || t < m - 6.0f || m == -INFINITY) ? fmaxf(t - 8.0f, m + __builtin_amdgcn_logf(sum) - 60.0f) : m;
+}
+
 // the keys [first, first + 32) that a row sees, of those before `end`: bit k for key first + k.  pos: the row's position; seen: its drafts (those outside its window left out)
 __device__ __forceinline__ uint32_t kv_below(int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1; }
 __device__ __forceinline__ uint32_t kv_visible(const KvAttnArgs& a, const KvRange& rg, int first, int end, int pos, uint64_t seen) {

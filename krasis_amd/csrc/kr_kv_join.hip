@@ -16,7 +16,7 @@ template <bool H, bool FEW> __global__ void __launch_bounds__(256) kr_kv_join_ke
             float top = -INFINITY, den = 0.0f; float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const float* sp = stats + ((size_t)first * bm + r) * 2; const float* wp = a.ws + ((size_t)first * bm + r) * dim + d;
             const size_t next = (size_t)step * bm;
-            for (int s0 = 0; s0 < it.nsplit; s0 += 4) {       // four shares at a time, measured from the largest maximum so far
+            for (int s0 = 0; s0 < it.nsplit; s0 += 4) {       // four shares at a time, measured from the largest reference so far
                 float ms[4], ls[4]; float4 x[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {

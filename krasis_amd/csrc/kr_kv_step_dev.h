@@ -4,7 +4,7 @@
 // Keys and values go from the pages to registers once, converted there to bf16 (exact, kr_kv_dev.h), and meet the queries in v_mfma_f32_16x16x32:
 //   S^T[key][row] = K Q^T    first operand: 16 key rows; a lane holds a quarter of a row, so a microscaled row costs it one scale and loads of 16 bytes
 //   O^T[d][row] += V^T P^T   a lane holds 8 keys and c neighbouring columns; byte permutes make them the columns' fragments
-// A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a running maximum and sum per row, and
+// A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a reference and a sum per row, and
 // meet in LDS.  Weights are rounded to the products' type, half a step of 2^-8 in bf16, as far as the result is rounded itself; f16 queries over pages that become bf16, and their weights, are
 // taken as two bf16 pieces (16 bits).
 // Measured: 32 requests of up to 8192 tokens at eight bits (142 MB) 30.5 us, 4.7 TB/s, two of 131071 and 100003 at four bits (126 MB) 29 us, 4.3 TB/s; 97 tokens of a chat 7 us, which is one
@@ -182,8 +182,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
 #pragma unroll
                 for (int i = 0; i < 4; i++) if (!(ok >> (16 * b + i) & 1)) st[b][i] = -INFINITY;
         }
-        // Weights from a reference, exp2(s - m): a row's first maximum in this wave, which moves, with what was summed so far, when a lane's sum gets out of the numbers' range (f16 ends at
-        // 2^16, bf16 and 32 bits are far from their end), and until the row has seen its first key.  NaN scores move nothing and are in the sums.
+        // Weights from a reference of the row in this wave (kr_kv_dev.h), which hardly ever moves.  NaN scores move nothing and are in the sums.
         u32x4 pf[NP];
         float hs = 0.0f;
         auto weigh = [&]() {
@@ -198,15 +197,17 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
             }
         };
         weigh();
-        if (__any(hs > most)) {
+        if (__any(kv_out_of_bounds<HM>(hs, most))) {
             float t = st[0][0];
 #pragma unroll
             for (int i = 1; i < 8; i++) t = fmaxf(t, st[i >> 2][i & 3]);
             t = fmaxf(t, __shfl_xor(t, 16)); t = fmaxf(t, __shfl_xor(t, 32));
-            const float mn = fmaxf(m, t * scale);
+            float sum = l;
+            if constexpr (HM) { sum += __shfl_xor(sum, 16); sum += __shfl_xor(sum, 32); }
+            const float mn = kv_reference<HM>(m, t * scale, sum);
             base = mn == -INFINITY ? 0.0f : mn;
             const float f = __builtin_amdgcn_exp2f(m - base);
-            m = mn; l *= f; most = mn == -INFINITY ? -1.0f : HM ? 8192.0f : 1073741824.0f;
+            m = mn; l *= f; most = kv_most<HM>(mn);
 #pragma unroll
             for (int j = 0; j < DIM / 16; j++) acc[j] *= f;
             weigh();
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
         for (; c + WAVES < c1; c += WAVES) tile(c, std::integral_constant<bool, true>());
         tile(c, std::integral_constant<bool, false>());
     }
-    // ---- the waves' states meet: [waves][16][DIM + 4] sums | [waves][16] maxima | [waves][16] denominators | [16] maximum | [16] denominator
+    // ---- the waves' states meet: [waves][16][DIM + 4] sums | [waves][16] references | [waves][16] denominators | [16] largest reference | [16] denominator
     constexpr int VS = DIM + 4;
     float* ml = kvs_lds_ + WAVES * 16 * VS; float* dl = ml + WAVES * 16; float* mt = dl + WAVES * 16; float* dt = mt + 16;
     l += __shfl_xor(l, 16); l += __shfl_xor(l, 32);

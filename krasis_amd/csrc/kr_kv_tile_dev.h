@@ -6,8 +6,8 @@
 //   O^T[d][row] += V^T P^T   the weights go from the accumulators to the operand in place (the order of keys within a product is free); V's columns come from the transposing LDS read
 // One or two waves share a SIMD, so a wave's own work has to overlap: the scores of the next half tile are multiplied while the weights of this one are formed, and the maxima of the
 // next half and the coming tiles' conversion go under the product with V; the first fragments of each product are read from LDS under the one before.
-// Weights are measured from a reference, exp2(s - m): a row's first maximum, which moves only when a half tile's sum of weights gets out of the numbers' range (their precision does not
-// depend on it).  No maxima are formed on the way, and O is hardly ever rescaled.
+// Weights are measured from a reference of the row (kr_kv_dev.h) that moves only when a half tile's sum of weights gets out of bounds.  No maxima are formed on the way, and O is hardly ever
+// rescaled.
 // Measured: two prompts of 8192 and 3001 tokens (64 / 4 heads of 128, eight bits) 1.03 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 46 % busy at the 1.9 GHz that its
 // power leaves; portions with heads of 256 channels over f16 pages 863 TFLOP/s, one wave a SIMD, 4.7 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
 // tile of 128 channels 1.3 us alone: short sequences are bound by that.
@@ -233,18 +233,20 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
 #pragma unroll
         for (int i = 0; i < 16; i++) if (!(ok >> ((i & 3) + 8 * (i >> 2)) & 1)) s[i] = -INFINITY;
     };
-    // The weights stand when no sum of a half tile is out of bounds (f16 ends at 2^16, bf16 and 32 bits are far from their end); else, and until a row has seen its first key, the
-    // references move to the maxima, and what was summed so far with them.  NaN scores move nothing and are in the sums.
+    // The weights stand when no sum of a half tile is out of bounds; else, and until a row has seen its first key, the references move, and what was summed so far with them.  NaN scores
+    // move nothing and are in the sums.
     auto settle = [&](const kv_f16& s) {
-        if (__any(hs > most)) {
+        if (__any(kv_out_of_bounds<HM>(hs, most))) {
             float t = s[0];
 #pragma unroll
             for (int i = 1; i < 16; i++) t = fmaxf(t, s[i]);
             t = fmaxf(t, __shfl_xor(t, 32)) * scale;
-            const float mn = fmaxf(m, t);
+            float sum = l;
+            if constexpr (HM) sum += __shfl_xor(sum, 32);
+            const float mn = kv_reference<HM>(m, t, sum);
             base = mn == -INFINITY ? 0.0f : mn;
             const float f = __builtin_amdgcn_exp2f(m - base);
-            m = mn; l *= f; most = mn == -INFINITY ? -1.0f : HM ? 8192.0f : 1073741824.0f;
+            m = mn; l *= f; most = kv_most<HM>(mn);
 #pragma unroll
             for (int d = 0; d < DB; d++)
 #pragma unroll

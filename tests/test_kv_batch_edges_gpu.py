@@ -94,3 +94,49 @@ def test_infinite_keys_draw_everything_or_nothing(fmt):
     got = batch.attend(0, q)
     out = agrees(got, q, cache, fmt, states, counts, 2.0 ** -8)
     assert bool(out[:, :2].isfinite().all()) and bool(out[:, 2:].isnan().all() if fmt == "mx8" else out[:, 2:].isfinite().all())
+
+
+# ---------------------------------------------------------------------------------------------------------------- weights far apart
+def scored(cache, fmt, states, counts, heads, dim, dtype, score, value, seed=5):
+    """keys whose products with every query are score(positions) and a little, values value(positions) in all channels; the queries, for scale 1"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kvh = cache.num_kv_heads
+    for s in states:
+        n = s.seq_len
+        pos = torch.arange(n, device="cuda")
+        k = 0.05 * torch.randn((n, kvh, dim), generator=g, device="cuda")
+        k[:, :, 2] = (score(pos, n) / 8)[:, None]
+        v = value(pos, n)[:, None, None] * (1 + 0.25 * torch.rand((n, kvh, dim), generator=g, device="cuda"))
+        page = torch.tensor(s.pages, device="cuda")[pos // cache.page_size]
+        cache.k_cache[0, page, pos % cache.page_size] = k.to(DTYPES[fmt]); cache.v_cache[0, page, pos % cache.page_size] = v.to(DTYPES[fmt])
+    q = torch.randn((sum(counts), heads, dim), generator=g, device="cuda")
+    q[:, :, 2] = 8.0
+    return q.to(dtype)
+
+
+@pytest.mark.parametrize("gap", [12, 17, 20, 24])
+@pytest.mark.parametrize("place", ["first", "middle", "three"])
+@pytest.mark.parametrize("dim,lens,counts", [(64, [4096], [1]), (128, [300, 20000], [1, 1]), (256, [700, 5000], [4, 1]), (64, [4500, 77], [40, 33]), (128, [2049, 9000], [64, 20]), (256, [3000], [70])])
+def test_keys_far_under_one_that_draws_nearly_all(dim, lens, counts, place, gap):
+    """f16 pages, where keys weigh exp(-gap) of one whose value is next to nothing: together they are the result.  A weight is an f16 number next to a reference, 2^8 at the largest of its half
+    tile or more: 32 keys beside the large one are off by 2^-25 of 2^8 of its weight, or all of their own; the others by half a step of 2^-11."""
+    cache = make_cache(2, dim, "f16", pages_for(lens, 16))
+    fill(cache, "f16", 1)
+    batch, states = batch_of(cache, lens, counts)
+    stored_poison(cache, "f16", states)
+    at = {"first": lambda p, n: p == 0, "middle": lambda p, n: p == n // 2, "three": lambda p, n: (p == 5) | (p == n // 3) | (p == n // 2)}[place]
+    q = scored(cache, "f16", states, counts, 4, dim, torch.float16, lambda p, n: torch.where(at(p, n), float(gap), 0.0), lambda p, n: torch.where(at(p, n), 0.0, 256.0))
+    got = batch.attend(0, q, scale=1.0)
+    beside = 32 * (3 if place == "three" else 1)
+    out = agrees(got, q, cache, "f16", states, counts, 2.0 ** -11, scale=1.0, few=beside * min(2.0 ** -33, math.exp(4 - gap)) * 320.0)
+    assert float(out.abs().min()) > 0
+
+
+@pytest.mark.parametrize("dim,lens,counts", [(64, [3000], [1]), (128, [2000, 700], [2, 40])])
+def test_scores_that_go_up_and_down(dim, lens, counts):
+    """f16 pages: scores that fall and rise by 40 natural units over the sequence, small values where the weights are; what is far under the largest weight has no part"""
+    cache = make_cache(2, dim, "f16", pages_for(lens, 16))
+    fill(cache, "f16", 1)
+    batch, states = batch_of(cache, lens, counts)
+    q = scored(cache, "f16", states, counts, 4, dim, torch.float16, lambda p, n: 20.0 * torch.cos(p * (9.0 / n)), lambda p, n: 1.0 + 0.1 * (p % 7))
+    agrees(batch.attend(0, q, scale=1.0), q, cache, "f16", states, counts, 2.0 ** -11, scale=1.0)
