@@ -145,13 +145,14 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& i
 // f16 weights (HM) are subnormal numbers below 2^-14 and end at 2^16.  The reference is 2^-8 of the largest weight it was taken from, moves up when a sum passes 2^15, and down again when it
 // falls under 2^-6: a key may draw nearly all attention and be worth nothing, and the many far under it are the result.  So the largest weight of a tile's keys is 2^-10 at least, the others are
 // off by 2^-25 at most.  It stays within 2^60 of what was summed, where 32-bit sums of 16-bit numbers have their end far away.
-// bf16 weights have the range of 32 bits, their sums are of no concern up to 2^30.
+// bf16 weights have the range of 32 bits.  The reference is 2^8 times the largest weight it was taken from, and moves up when a sum passes 1: no weight is over 1, so that values up to the end of
+// the numbers have no larger sums than the definition gives them, and weights end at 2^-118 of the largest.
 template <bool HM> __device__ __forceinline__ bool kv_out_of_bounds(float sum, float most) { return sum > most || (HM && sum < 0.015625f); }
 // most: -1 until the row has seen a key
-template <bool HM> __device__ __forceinline__ float kv_most(float m) { return m == -INFINITY ? -1.0f : HM ? 32768.0f : 1073741824.0f; }
+template <bool HM> __device__ __forceinline__ float kv_most(float m) { return m == -INFINITY ? -1.0f : HM ? 32768.0f : 1.0f; }
 // the reference after keys whose largest score is t; sum: all of the row's weights so far
 template <bool HM> __device__ __forceinline__ float kv_reference(float m, float t, float sum) {
-    if constexpr (!HM) return fmaxf(m, t);
+    if constexpr (!HM) return fmaxf(m, t + 8.0f);
     else return t != -INFINITY && (t > m + 8.0f || t < m - 6.0f || m == -INFINITY) ? fmaxf(t - 8.0f, m + __builtin_amdgcn_logf(sum) - 60.0f) : m;
 }
 

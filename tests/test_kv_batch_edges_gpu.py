@@ -140,3 +140,18 @@ def test_scores_that_go_up_and_down(dim, lens, counts):
     batch, states = batch_of(cache, lens, counts)
     q = scored(cache, "f16", states, counts, 4, dim, torch.float16, lambda p, n: 20.0 * torch.cos(p * (9.0 / n)), lambda p, n: 1.0 + 0.1 * (p % 7))
     agrees(batch.attend(0, q, scale=1.0), q, cache, "f16", states, counts, 2.0 ** -11, scale=1.0)
+
+
+# ---------------------------------------------------------------------------------------------------------------- values near the end of the numbers
+@pytest.mark.parametrize("rise", [6, 25, 29, 60])
+@pytest.mark.parametrize("dim,lens,counts", [(64, [300], [1]), (128, [300, 900], [1, 3]), (64, [300], [40]), (128, [300, 900], [70, 64]), (256, [500], [33])])
+def test_large_values_under_rising_scores(dim, lens, counts, rise):
+    """bf16 pages: values of 2^117 under scores that rise by `rise` powers of two, far behind the first keys.  No sum of weights times values passes the plain form's, at most 900 times 2^117."""
+    cache = make_cache(2, dim, "bf16", pages_for(lens, 16))
+    fill(cache, "bf16", 1)
+    batch, states = batch_of(cache, lens, counts)
+    stored_poison(cache, "bf16", states)
+    q = scored(cache, "bf16", states, counts, 4, dim, torch.bfloat16, lambda p, n: torch.where(p > n // 2, rise * math.log(2.0), 0.0), lambda p, n: torch.full(p.shape, 2.0 ** 117, device="cuda"))
+    got = batch.attend(0, q, scale=1.0)
+    out = agrees(got, q, cache, "bf16", states, counts, 2.0 ** -8, scale=1.0)
+    assert bool(out.isfinite().all()) and float(out.abs().max()) > 2.0 ** 116
