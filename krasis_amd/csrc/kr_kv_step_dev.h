@@ -5,8 +5,7 @@
 //   S^T[key][row] = K Q^T    first operand: 16 key rows; a lane holds a quarter of a row, so a microscaled row costs it one scale and loads of 16 bytes
 //   O^T[d][row] += V^T P^T   a lane holds 8 keys and c neighbouring columns; byte permutes make them the columns' fragments
 // A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a reference and a sum per row, and
-// meet in LDS.  Weights are rounded to the products' type, half a step of 2^-8 in bf16, as far as the result is rounded itself; f16 queries over pages that become bf16, and their weights, are
-// taken as two bf16 pieces (16 bits).
+// meet in LDS.  Over pages that become bf16 weights are two bf16 pieces (off by 2^-16), and so are f16 queries; over f16 pages weights are f16 (2^-11, as the result is rounded itself).
 // Measured: 32 requests of up to 8192 tokens at eight bits (142 MB) 30.5 us, 4.7 TB/s, two of 131071 and 100003 at four bits (126 MB) 29 us, 4.3 TB/s; 97 tokens of a chat 7 us, which is one
 // round trip after the other (arguments, plan, page table, keys).
 #pragma once
@@ -46,7 +45,7 @@ template <int DIM, int FMT, bool HQ, bool ONE>
 __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step_waves(DIM, FMT, HQ, ONE) / 4) kr_kv_step_kernel(const KvAttnArgs a) {
     constexpr int WAVES = kv_step_waves(DIM, FMT, HQ, ONE);
     constexpr bool HM = HQ && FMT == 0;                       // f16 products
-    constexpr int NP = HQ && !HM ? 2 : 1;                     // bf16 pieces of an f16 query and of its weights
+    constexpr int NP = HQ && !HM ? 2 : 1, NW = HM ? 1 : 2;    // pieces of a query, of a weight
     constexpr int BITS = FMT == 0 ? 16 : FMT == 1 ? 8 : 4, U = DIM / 32, KB = DIM / 4 * BITS / 8, KW = KB / 4;
     constexpr int C = KvsCols<DIM>::C, GROUPS = KvsCols<DIM>::GROUPS, VB = C * BITS / 8, VW = VB < 4 ? 1 : VB / 4;
     constexpr int NB = DIM == 64 || DIM == 128 ? 1 : 2;       // blocks of 32 channels that a quarter of a row meets
@@ -183,7 +182,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
                 for (int i = 0; i < 4; i++) if (!(ok >> (16 * b + i) & 1)) st[b][i] = -INFINITY;
         }
         // Weights from a reference of the row in this wave (kr_kv_dev.h), which hardly ever moves.  NaN scores move nothing and are in the sums.
-        u32x4 pf[NP];
+        u32x4 pf[NW];
         float hs = 0.0f;
         auto weigh = [&]() {
             hs = 0.0f;
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
                 const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 1][2 * (e & 1)], scale, -base)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 1][2 * (e & 1) + 1], scale, -base));
                 const uint32_t w = kv_pack<HM>(p0, p1);
                 pf[0][e] = w;
-                if constexpr (NP == 2) { pf[1][e] = kv_rest(p0, p1, w); hs += p0 + p1; }
+                if constexpr (NW == 2) { pf[1][e] = kv_rest(p0, p1, w); hs += p0 + p1; }
                 else hs = kv_sum2<HM>(w, hs);
             }
         };
@@ -215,8 +214,10 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
         l += hs;
         constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;
         // A value that is not finite may belong to a key that some rows do not see, and 0 times it would not be 0.  Rows of one token see the same keys: what they do not see becomes 0.
-        // Else such values are looked for (in tiles that all rows see entirely, too: a weight may be too small for the numbers).
-        const bool look = !ONE && (hidden || it.cnt > 1);
+        // Else such values are looked for (in tiles that all rows see entirely, too: a weight may be too small for the numbers).  A weight's second piece is 0 or negative where the weight
+        // is not, so that infinities, which 16-bit pages may hold, meet the first one alone.
+        constexpr bool APART = FMT == 0 && NW == 2;
+        const bool look = APART || (!ONE && (hidden || it.cnt > 1));
         if constexpr (ONE) if (hidden) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -237,10 +238,11 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
 #pragma unroll
                 for (int i = 0; i < 8; i++) w[i] = kvs_two<FMT>(vn[i][g], e2, FMT == 0 ? 1.0f : scale_of(vsn[i][g]));
                 bool odd = false;
-                if (look) {
+                if (look) {                                   // all ones in a field, and one more: a carry into the sign's place of its number
+                    uint32_t bad = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) odd = odd || (w[i] & EXP) == EXP || (w[i] >> 16 & EXP) == EXP;
-                    odd = __any(odd);
+                    for (int i = 0; i < 8; i++) bad |= (w[i] & EXP * 0x10001u) + (EXP & -EXP) * 0x10001u;
+                    odd = __any((bad & 0x80008000u) != 0);
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -248,7 +250,12 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
                     u32x4 vf;
 #pragma unroll
                     for (int e = 0; e < 4; e++) vf[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], u ? 0x07060302u : 0x05040100u);
-                    if (odd) {                                // such values apart: whether a row sees one, by kind
+                    u32x4 vl = vf;                            // what a weight's second piece meets
+                    if (ONE && odd) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) { const uint32_t bad = ((vf[e] & EXP * 0x10001u) + (EXP & -EXP) * 0x10001u) & 0x80008000u; vl[e] = vf[e] & ~((bad << 1) - (bad >> 15)); }
+                    }
+                    if (!ONE && odd) {                        // such values apart: whether a row sees one, by kind
                         u32x4 see;                            // ones where the row sees the key, as a fragment
 #pragma unroll
                         for (int e = 0; e < 4; e++) see[e] = (ok >> ((e >> 1) * 16 + 2 * (e & 1)) & 1 ? UNIT : 0u) | (ok >> ((e >> 1) * 16 + 2 * (e & 1) + 1) & 1 ? UNIT << 16 : 0u);
@@ -270,10 +277,10 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
 #pragma unroll
                             for (int i = 0; i < 4; i++) if (n[i] > 0.0f) acc[j][i] += k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
                         }
-                        vf = keep;
+                        vf = vl = keep;
                     }
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; p--) acc[j] = kvs_mfma<HM>(vf, pf[p], acc[j]);
+                    if constexpr (NW == 2) acc[j] = kvs_mfma<HM>(vl, pf[1], acc[j]);
+                    acc[j] = kvs_mfma<HM>(vf, pf[0], acc[j]);
                 }
             }
         __builtin_amdgcn_sched_barrier(0);

@@ -155,3 +155,14 @@ def test_large_values_under_rising_scores(dim, lens, counts, rise):
     got = batch.attend(0, q, scale=1.0)
     out = agrees(got, q, cache, "bf16", states, counts, 2.0 ** -8, scale=1.0)
     assert bool(out.isfinite().all()) and float(out.abs().max()) > 2.0 ** 116
+
+
+# ---------------------------------------------------------------------------------------------------------------- how near
+@pytest.mark.parametrize("fmt,dim,lens,counts", [("bf16", 128, [97, 500], [1, 1]), ("mx8", 128, [97, 9000], [1, 1]), ("mx4", 64, [3000], [2]), ("e4m3", 256, [700, 90], [1, 2]), ("mx4", 128, [2000], [1])])
+def test_single_tokens_weigh_in_sixteen_bits(fmt, dim, lens, counts):
+    """sequences of at most 16 rows, bf16 queries: weights are two bf16 pieces, off by 2^-8 of 2^-8"""
+    cache = make_cache(2, dim, fmt, pages_for(lens, 16))
+    fill(cache, fmt, 3)
+    batch, states = batch_of(cache, lens, counts)
+    q = rows(sum(counts), 8, dim, torch.bfloat16, 4)
+    agrees(batch.attend(0, q), q, cache, fmt, states, counts, 2.0 ** -16)
