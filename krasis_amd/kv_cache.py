@@ -172,7 +172,7 @@ class SequenceKVState:
     def unpage(self, paged_layer: torch.Tensor, out_dtype: Optional[torch.dtype] = torch.float16) -> torch.Tensor:
         """rows 0 .. seq_len-1 of one layer's paged tensor `[pages, page_size, ...]` as a flat `[seq_len, prod(...)]` tensor; out_dtype None keeps the
         page dtype (E4M3 bytes for a store that runs an FP8 cache), else the exact widening the reference applies (`.to(torch.float16)`)."""
-        if self.cache.kv_format is not None:
+        if getattr(self.cache, "kv_format", None) is not None:
             raise ValueError("microscaled pages hold codes that mean nothing without their scales: KVBatch.stored(cache, [state]).read(layer)")
         if self.seq_len == 0:
             return paged_layer.new_zeros((0, int(paged_layer[0, 0].numel())), dtype=out_dtype or paged_layer.dtype)
@@ -190,9 +190,10 @@ def unpage_into_store(store, seq_state: SequenceKVState, layer_map, kv_max_seq: 
     import numpy as np
     cache = seq_state.cache
     fp8_store = bool(getattr(store, "_kv_fp8", False))
-    if cache.kv_format is not None and fp8_store:
+    microscaled = getattr(cache, "kv_format", None) is not None       # a caller's own cache object may know nothing of it
+    if microscaled and fp8_store:
         raise ValueError("microscaled pages go to a store with an FP16 cache (set_kv_dtype(False)): E4M3 without scales does not hold their values")
-    batch = KVBatch.stored(cache, [seq_state]) if cache.kv_format is not None and any(off is not None for off in layer_map) else None
+    batch = KVBatch.stored(cache, [seq_state]) if microscaled and any(off is not None for off in layer_map) else None
     ks, vs, held = [], [], []
     for off in layer_map:
         if off is None:

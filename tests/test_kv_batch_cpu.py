@@ -183,3 +183,25 @@ def test_sequences_may_write_to_different_slots_of_a_page():
     assert plan_of(cache, [a, b], [7, 2])[5] == 0                   # a's at 4 to 10
     a.pages = tuple(a.pages)
     assert plan_of(cache, [a], [2])[5] == 1
+
+
+def test_a_callers_own_cache_object_is_unpaged_as_before():
+    from krasis_amd.kv_cache import SequenceKVState, unpage_into_store
+    made = make_cache(2, 64, "f16", 8, device="cpu")
+
+    class Own:                                                      # the surface that these two read, without what PagedKVCache has gained
+        page_size, attention_type, kv_dtype, combined = made.page_size, "gqa", torch.float16, False
+        k_cache, v_cache = made.k_cache, made.v_cache
+        alloc_pages = made.alloc_pages
+
+        def get_gqa_layer_caches(self, off): return self.k_cache[off], self.v_cache[off]
+    made.k_cache.copy_(torch.arange(made.k_cache.numel()).view(made.k_cache.shape) % 1000)
+    s = SequenceKVState(Own(), 0); s.ensure_capacity(20); s.advance(20)
+    want = torch.stack([made.k_cache[0, s.pages[p // 16], p % 16].flatten() for p in range(20)])
+    assert torch.equal(s.unpage(made.k_cache[0]), want)
+
+    class Store:
+        def set_decode_state(self, *args): self.args = args
+    store = Store()
+    (k, v), = unpage_into_store(store, s, [None, 0], 32)
+    assert store.args[0] == 20 and torch.equal(torch.from_numpy(k.view("float16"))[:20], want) and not v.any()
