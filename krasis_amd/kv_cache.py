@@ -394,7 +394,8 @@ class KVBatch:
 
     def commit(self) -> None:
         """The new tokens are part of the sequences from here on."""
-        self._finish()
+        self._unfinished()
+        self._done = True
         for s, c in zip(self.states, self.counts):
             s.advance(c)
 
@@ -409,7 +410,7 @@ class KVBatch:
                 raise ValueError(f"path {p}: rising numbers of {c} drafts")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("keep copies its paths to the device: not during a capture")
-        self._finish()
+        self._unfinished()
         start, src, dst, at, slots = [0], [], [], 0, self._host[len(self._host) - self.rows:].tolist()
         for p, c in zip(paths, self.counts):
             for to, i in enumerate(p):
@@ -420,15 +421,15 @@ class KVBatch:
             n = len(start)
             moves = torch.tensor(start + src + dst, dtype=torch.int32, device=self.device)
             self._call(self._lib.kr_kv_move, self._layer(0), self.cache.num_layers, len(paths), moves.data_ptr(), moves.data_ptr() + 4 * n, moves.data_ptr() + 4 * (n + len(src)))
+        self._done = True                                # not before: a launch that is refused leaves everything as it was
         for s, p in zip(self.states, paths):
             s.advance(len(p))
 
-    def _finish(self) -> None:
+    def _unfinished(self) -> None:
         if self._done:
             raise RuntimeError("the batch's tokens are part of their sequences already")
         if self._lens != [s.seq_len for s in self.states]:
             raise RuntimeError("a sequence has changed since the batch was made: its new tokens are not where it ends")
-        self._done = True
 
 
 def plan_of(cache: PagedKVCache, states: Sequence[SequenceKVState], counts: Sequence[int], stored: bool = False) -> torch.Tensor:

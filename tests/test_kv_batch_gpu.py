@@ -476,3 +476,28 @@ def test_a_batch_ends_on_the_sequences_that_it_was_made_for(end):
     with pytest.raises(RuntimeError, match="has changed"):
         late.commit() if end == "commit" else late.keep([[0]])
     assert b.seq_len == 0
+
+
+def test_paths_whose_move_was_refused_are_still_to_be_kept(monkeypatch):
+    from krasis_amd.kv_cache import KVBatch
+    cache = make_cache(2, 64, "mx8", 20)
+    fill(cache, "mx8", 1)
+    a, b = sequences(cache, [5, 7])
+    batch, layer = KVBatch(cache, [a, b], [4, 2]), (cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale)
+    slot = lambda s, p: (0, s.pages[p // 16], p % 16)
+    want = [[t.view(torch.uint8)[slot(s, p)].clone() for s, p in ((a, 6), (a, 8), (b, 7))] for t in layer]
+
+    def refuse(*args): raise ValueError("refused")
+    with monkeypatch.context() as m:
+        m.setattr(batch, "_call", refuse)
+        with pytest.raises(ValueError, match="refused"):
+            batch.keep([[1, 3], [0]])
+    assert (a.seq_len, b.seq_len) == (5, 7)
+    batch.keep([[1, 3], [0]])
+    assert (a.seq_len, b.seq_len) == (7, 8)
+    for t, rows_ in zip(layer, want):
+        for got, w in zip((slot(a, 5), slot(a, 6), slot(b, 7)), rows_):
+            assert torch.equal(t.view(torch.uint8)[got], w)
+    for again in (batch.commit, lambda: batch.keep([[0], [0]])):
+        with pytest.raises(RuntimeError, match="already"):
+            again()
