@@ -1109,12 +1109,15 @@ int kr_moe_prefill_set(kr_engine* e, int layer, const void* x_bf16, const int32_
     const KrPfTiles most = kr_pf_tiles(L.w13.view(), L.w2.view(), CH, (long)np, E, beside);
     const size_t gu_rows = kr_pf_gu_rows(most, np, E), sgu_rows = joins(most, CH) ? std::min((size_t)CH, gu_rows / topk) : CH;
     const size_t n_i32 = 3 * (size_t)E + 3 * (size_t)max_tiles + 4 + 2 * np;
+    // both digits of the hidden rows in one allocation, which takes whole pages of 2 MB
+    const size_t hbytes = (np * I + 255) / 256 * 256, sbytes = ((size_t)CH * SI + 255) / 256 * 256;
     if (P.i32.ensure(n_i32 * 4) || P.xh.ensure((size_t)CH * H) || P.xl.ensure((size_t)CH * H) || P.xs.ensure((size_t)CH * (H / 128) * 4) ||
-        P.gu.ensure(gu_rows * 2 * I * 4) || P.hh.ensure(np * I) || P.hl.ensure(np * I) || P.hs.ensure(np * (I / 128) * 4) || P.eo.ensure(np * H * 4))
+        P.gu.ensure(gu_rows * 2 * I * 4) || P.hh.ensure(2 * hbytes) || P.hs.ensure(np * (I / 128) * 4) || P.eo.ensure(np * H * 4))
         return kr_fail(KR_ERR_HIP, "hipMalloc of prefill scratch failed");
-    if (use_shared && (P.sgu.ensure(sgu_rows * 2 * SI * 4) || P.shh.ensure((size_t)CH * SI) || P.shl.ensure((size_t)CH * SI) ||
+    if (use_shared && (P.sgu.ensure(sgu_rows * 2 * SI * 4) || P.shh.ensure(2 * sbytes) ||
                        P.shs.ensure((size_t)CH * (SI / 128) * 4) || P.seo.ensure((size_t)CH * H * 4)))
         return kr_fail(KR_ERR_HIP, "hipMalloc of prefill scratch failed");
+    int8_t* const hh = (int8_t*)P.hh.p; int8_t* const hl = hh + hbytes; int8_t* const shh = (int8_t*)P.shh.p; int8_t* const shl = use_shared ? shh + sbytes : nullptr;
     int* ib = (int*)P.i32.p;
     KrPfSort so{};
     so.counts = ib; so.offsets = ib + E; so.cursor = ib + 2 * E; ib += 3 * E;
@@ -1133,17 +1136,17 @@ int kr_moe_prefill_set(kr_engine* e, int layer, const void* x_bf16, const int32_
         KrPfDense d13{}, d2{};
         if (use_shared) {
             d13 = KrPfDense{L.sw13.view(), (const uint32_t*)L.sw13.wsum.p, (const int8_t*)P.xh.p, (const int8_t*)P.xl.p, (const float*)P.xs.p, mc, (float*)P.sgu.p, 2 * SI};
-            d2 = KrPfDense{L.sw2.view(), (const uint32_t*)L.sw2.wsum.p, (const int8_t*)P.shh.p, (const int8_t*)P.shl.p, (const float*)P.shs.p, mc, (float*)P.seo.p, H};
+            d2 = KrPfDense{L.sw2.view(), (const uint32_t*)L.sw2.wsum.p, shh, shl, (const float*)P.shs.p, mc, (float*)P.seo.p, H};
         }
         const bool join = joins(cut, mc);
         auto shared_gemm = [&](const KrPfDense& d) { kr_launch_pf_gemm(d.m, d.wsum, d.a_hi, d.a_lo, d.a_scale, nullptr, topk, 0, 0, d.rows, d.out, d.out_ld, st); };
-        auto shared_act = [&] { kr_launch_pf_act((const float*)P.sgu.p, mc, SI, 2 * SI, act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, (int8_t*)P.shh.p, (int8_t*)P.shl.p,
+        auto shared_act = [&] { kr_launch_pf_act((const float*)P.sgu.p, mc, SI, 2 * SI, act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, shh, shl,
                                                  (float*)P.shs.p, st); };
-        const KrPfAct f13{act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, (int8_t*)P.hh.p, (int8_t*)P.hl.p, (float*)P.hs.p};
-        const KrPfAct fs13{act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, (int8_t*)P.shh.p, (int8_t*)P.shl.p, (float*)P.shs.p};
+        const KrPfAct f13{act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, hh, hl, (float*)P.hs.p};
+        const KrPfAct fs13{act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, shh, shl, (float*)P.shs.p};
         kr_launch_pf_w13_act(L.w13.view(), (const uint32_t*)L.w13.wsum.p, (const int8_t*)P.xh.p, (const int8_t*)P.xl.p, (const float*)P.xs.p, &so, topk, (float*)P.gu.p, mc * topk, f13, st,
                              var_rows, cut, join ? &d13 : nullptr, &fs13);
-        kr_launch_pf_gemm(L.w2.view(), (const uint32_t*)L.w2.wsum.p, (const int8_t*)P.hh.p, (const int8_t*)P.hl.p, (const float*)P.hs.p, &so, topk, 0,
+        kr_launch_pf_gemm(L.w2.view(), (const uint32_t*)L.w2.wsum.p, hh, hl, (const float*)P.hs.p, &so, topk, 0,
                           cut.max_tiles, 0, (float*)P.eo.p, H, st, 0, 0, var_rows, &cut, join ? &d2 : nullptr);
         if (use_shared && !join) { shared_gemm(d13); shared_act(); shared_gemm(d2); }
         kr_launch_pf_combine((const float*)P.eo.p, so.pair_row, wc, mc, topk, H, use_shared ? (const float*)P.seo.p : nullptr, e->cfg.routed_scaling_factor,
@@ -1171,10 +1174,11 @@ int kr_moe_prefill_rows(kr_engine* e, int layer, const void* rows_bf16, const in
     const size_t np = (size_t)CH;
     const int max_tiles = (int)(np / 16) + E + 1;      // (strips of 16 rows are the smallest, kr_pf_tiles)
     const size_t gu_rows = kr_pf_gu_rows(kr_pf_tiles(L.w13.view(), L.w2.view(), CH, (long)np, E, true), np, E);      // (see kr_moe_prefill_set)
-    const size_t n_i32 = 3 * (size_t)E + 3 * (size_t)max_tiles + 4 + 2 * np;
+    const size_t n_i32 = 3 * (size_t)E + 3 * (size_t)max_tiles + 4 + 2 * np, hbytes = (np * I + 255) / 256 * 256;
     if (P.i32.ensure(n_i32 * 4) || P.xh.ensure((size_t)CH * H) || P.xl.ensure((size_t)CH * H) || P.xs.ensure((size_t)CH * (H / 128) * 4) ||
-        P.gu.ensure(gu_rows * 2 * I * 4) || P.hh.ensure(np * I) || P.hl.ensure(np * I) || P.hs.ensure(np * (I / 128) * 4))
+        P.gu.ensure(gu_rows * 2 * I * 4) || P.hh.ensure(2 * hbytes) || P.hs.ensure(np * (I / 128) * 4))
         return kr_fail(KR_ERR_HIP, "hipMalloc of prefill scratch failed");
+    int8_t* const hh = (int8_t*)P.hh.p; int8_t* const hl = hh + hbytes;
     int* ib = (int*)P.i32.p;
     KrPfSort so{};
     so.counts = ib; so.offsets = ib + E; so.cursor = ib + 2 * E; ib += 3 * E;
@@ -1188,9 +1192,9 @@ int kr_moe_prefill_rows(kr_engine* e, int layer, const void* rows_bf16, const in
         kr_launch_pf_sort(lid + m0, mc, 1, E, so, st, cut);
         kr_launch_pf_quant_x((const uint16_t*)rows_bf16 + (size_t)m0 * H, mc, H, (int8_t*)P.xh.p, (int8_t*)P.xl.p, (float*)P.xs.p, st);
         const int var_rows = (long)mc < 48L * E;
-        const KrPfAct f13{act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, (int8_t*)P.hh.p, (int8_t*)P.hl.p, (float*)P.hs.p};
+        const KrPfAct f13{act_mode, e->cfg.swiglu_limit, e->cfg.activation_alpha, hh, hl, (float*)P.hs.p};
         kr_launch_pf_w13_act(L.w13.view(), (const uint32_t*)L.w13.wsum.p, (const int8_t*)P.xh.p, (const int8_t*)P.xl.p, (const float*)P.xs.p, &so, 1, (float*)P.gu.p, mc, f13, st, var_rows, cut);
-        kr_launch_pf_gemm(L.w2.view(), (const uint32_t*)L.w2.wsum.p, (const int8_t*)P.hh.p, (const int8_t*)P.hl.p, (const float*)P.hs.p, &so, 1, 0,
+        kr_launch_pf_gemm(L.w2.view(), (const uint32_t*)L.w2.wsum.p, hh, hl, (const float*)P.hs.p, &so, 1, 0,
                           cut.max_tiles, 0, (float*)((char*)out + (size_t)m0 * H * ob), H, st, 1, out_bf16, var_rows, &cut);
     }
     KR_HIP(hipGetLastError());
