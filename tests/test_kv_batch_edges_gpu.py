@@ -1,12 +1,13 @@
 """Operators over a caller's paged cache where numbers are hard: infinities, weights far below another, values near the end of the numbers, shares that are joined; the definition is
 tests/kv_reference.py."""
 import math
+import random
 
 import pytest
 import torch
 
 from tests.kv_reference import DTYPES, attend, make_cache, stored_rows, tolerance, visible
-from tests.test_kv_batch_gpu import fill, rows, sequences, stored_poison
+from tests.test_kv_batch_gpu import fill, rows, sequences, stored_poison, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -166,3 +167,60 @@ def test_single_tokens_weigh_in_sixteen_bits(fmt, dim, lens, counts):
     batch, states = batch_of(cache, lens, counts)
     q = rows(sum(counts), 8, dim, torch.bfloat16, 4)
     agrees(batch.attend(0, q), q, cache, fmt, states, counts, 2.0 ** -16)
+
+
+# ---------------------------------------------------------------------------------------------------------------- shares that are joined
+@pytest.mark.parametrize("fmt,dtype,dim,lens,counts,window,first", [
+    ("mx8", "bf16", 128, [4096, 4000, 3900, 4090, 4096, 3333, 4001, 4077], [12] * 8, 0, 0), ("mx8", "bf16", 128, [4096, 4000, 3900, 4090], [12, 3, 1, 12], 3000, 4), ("mx4", "f16", 64, [9001, 8000], [64, 60], 0, 0),
+    ("mx8", "bf16", 128, [9001, 8000], [64, 33], 5, 7000), ("f16", "f16", 128, [9001, 8700], [64, 40], 4000, 8), ("bf16", "bf16", 64, [20000], [4], 0, 0), ("bf16", "bf16", 64, [20000], [4], 3, 18000)])
+def test_trees_whose_sequences_are_shared_out(fmt, dtype, dim, lens, counts, window, first):
+    cache = make_cache(2, dim, fmt, pages_for(lens, 64), page=64)
+    fill(cache, fmt, 1, spread=1)
+    batch, states = batch_of(cache, lens, counts)
+    stored_poison(cache, fmt, states)
+    trees = [tree(n, 3 + i) for i, n in enumerate(counts)]
+    q = rows(sum(counts), 8, dim, DTYPES[dtype], 4)
+    got = batch.attend_tree(0, q, trees, window=window, keep_first=first)
+    assert min(batch._need.values()) > 0                            # partial results, joined
+    weight = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11 if fmt == "f16" else 2.0 ** -16
+    agrees(got, q, cache, fmt, states, counts, weight, window=window, first=first, trees=trees)
+
+
+def test_two_streams_with_shares_each():
+    """calls on two streams at once, both with partial results of their own"""
+    lens, counts = [9000, 100, 400], [1, 1, 40]
+    cache = make_cache(2, 128, "mx8", pages_for(lens, 16))
+    fill(cache, "mx8", 1)
+    batch, _ = batch_of(cache, lens, counts)
+    q = rows(42, 16, 128, torch.bfloat16, 2)
+    calls = lambda: batch.attend(0, q), lambda: batch.attend(0, q, window=4000, keep_first=4)
+    want = [c() for c in calls]
+    assert len(batch._need) == 2 and min(batch._need.values()) > 0
+    torch.cuda.synchronize()
+    streams, got = (torch.cuda.Stream(), torch.cuda.Stream()), ([], [])
+    for _ in range(20):
+        for s, c, g in zip(streams, calls, got):
+            with torch.cuda.stream(s):
+                g.append(c())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
+def test_a_first_call_may_be_captured():
+    """none of the kernels has run before in this form: what a first launch needs is no stream's work"""
+    lens, counts = [5000, 70], [1, 33]
+    for fmt, dtype, dim in (("mx4", torch.float16, 192), ("e4m3", torch.float16, 96)):
+        cache = make_cache(1, dim, fmt, pages_for(lens, 128), page=128)
+        fill(cache, fmt, 1)
+        batch, states = batch_of(cache, lens, counts)
+        q, k = rows(34, 5, dim, dtype, 2), rows(34, 1, dim, dtype, 3)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            batch.write(0, k, k)
+            got = batch.attend(0, q)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            agrees(got, q, cache, fmt, states, counts, 2.0 ** -16)
+            assert torch.equal(got, batch.attend(0, q))
