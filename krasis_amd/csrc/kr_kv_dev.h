@@ -148,12 +148,17 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& i
 // bf16 weights have the range of 32 bits.  The reference is 2^8 times the largest weight it was taken from, and moves up when a sum passes 1: no weight is over 1, so that values up to the end of
 // the numbers have no larger sums than the definition gives them, and weights end at 2^-118 of the largest.
 template <bool HM> __device__ __forceinline__ bool kv_out_of_bounds(float sum, float most) { return sum > most || (HM && sum < 0.015625f); }
-// most: -1 until the row has seen a key
-template <bool HM> __device__ __forceinline__ float kv_most(float m) { return m == -INFINITY ? -1.0f : HM ? 32768.0f : 1.0f; }
+// Weights are worked out as exp2(fma(product, scale, -m)), and once more where the reference moves: as exp2(score - m) of scores rounded to 32 bits, as m is.  Past 2^20 the rounding of m is no
+// longer small, and would be all that a weight from the fma is made of past 2^27: there all weights are worked out twice.
+// most: -1, which every sum passes, until the row has seen a key, and for references past 2^20
+template <bool HM> __device__ __forceinline__ float kv_most(float m) { return fabsf(m) > 1048576.0f ? -1.0f : HM ? 32768.0f : 1.0f; }
 // the reference after keys whose largest score is t; sum: all of the row's weights so far
 template <bool HM> __device__ __forceinline__ float kv_reference(float m, float t, float sum) {
     if constexpr (!HM) return fmaxf(m, t + 8.0f);
-    else return t != -INFINITY && (t > m + 8.0f || t < m - 6.0f || m == -INFINITY) ? fmaxf(t - 8.0f, m + __builtin_amdgcn_logf(sum) - 60.0f) : m;
+    else {
+        const float low = t - 8.0f;                          // past 2^27 the numbers lie 16 apart
+        return t != -INFINITY && (t - m > 8.0f || m - t > 6.0f) ? fmaxf(t - low > 8.0f ? t : low, m + __builtin_amdgcn_logf(sum) - 60.0f) : m;
+    }
 }
 
 // the keys [first, first + 32) that a row sees, of those before `end`: bit k for key first + k.  pos: the row's position; seen: its drafts (those outside its window left out)

@@ -184,18 +184,19 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
         // Weights from a reference of the row in this wave (kr_kv_dev.h), which hardly ever moves.  NaN scores move nothing and are in the sums.
         u32x4 pf[NW];
         float hs = 0.0f;
-        auto weigh = [&]() {
+        auto weigh = [&](auto AGAIN) {
             hs = 0.0f;
+            auto from = [&](float s) { return __builtin_amdgcn_exp2f(AGAIN ? s * scale - base : __builtin_fmaf(s, scale, -base)); };
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 1][2 * (e & 1)], scale, -base)), p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 1][2 * (e & 1) + 1], scale, -base));
+                const float p0 = from(st[e >> 1][2 * (e & 1)]), p1 = from(st[e >> 1][2 * (e & 1) + 1]);
                 const uint32_t w = kv_pack<HM>(p0, p1);
                 pf[0][e] = w;
                 if constexpr (NW == 2) { pf[1][e] = kv_rest(p0, p1, w); hs += p0 + p1; }
                 else hs = kv_sum2<HM>(w, hs);
             }
         };
-        weigh();
+        weigh(std::integral_constant<bool, false>());
         if (__any(kv_out_of_bounds<HM>(hs, most))) {
             float t = st[0][0];
 #pragma unroll
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
             m = mn; l *= f; most = kv_most<HM>(mn);
 #pragma unroll
             for (int j = 0; j < DIM / 16; j++) acc[j] *= f;
-            weigh();
+            weigh(std::integral_constant<bool, true>());
         }
         l += hs;
         constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;

@@ -176,12 +176,17 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
         const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) kvt_h4*)(va + 8 * LDV)));
         return u32x4{x.x, x.y, y.x, y.y};
     };
+    using yes = std::integral_constant<bool, true>; using no = std::integral_constant<bool, false>;
     // The weights of scores 2 e, 2 e + 1 of a half tile, and the lane's sum of them as they enter the product, in four stages that different pairs are at in one step: each waits
     // for the one before it, and a wave issues in order.  The empty asm statements keep a stage in its step.
     float x0[4], x1[4];
-    auto stage = [&](const kv_f16& s, int e, int k) {
+    auto stage = [&](const kv_f16& s, int e, int k, auto AGAIN) {
         float& a0 = x0[e & 3]; float& a1 = x1[e & 3];
-        if (k == 0) { a0 = __builtin_fmaf(s[2 * e], scale, -base); a1 = __builtin_fmaf(s[2 * e + 1], scale, -base); asm volatile("" : "+v"(a0), "+v"(a1)); }
+        if (k == 0) {
+            if constexpr (AGAIN) { a0 = s[2 * e] * scale - base; a1 = s[2 * e + 1] * scale - base; }
+            else { a0 = __builtin_fmaf(s[2 * e], scale, -base); a1 = __builtin_fmaf(s[2 * e + 1], scale, -base); }
+            asm volatile("" : "+v"(a0), "+v"(a1));
+        }
         else if (k == 1) { a0 = __builtin_amdgcn_exp2f(a0); a1 = __builtin_amdgcn_exp2f(a1); asm volatile("" : "+v"(a0), "+v"(a1)); }
         else if (k == 2) {
             uint32_t w = kv_pack<HM>(a0, a1);
@@ -195,9 +200,9 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
             asm volatile("" : "+v"(hs));
         }
     };
-    auto weigh = [&](const kv_f16& s, int t) {                // pair t begins, those before it go on; t = 0 .. 10
+    auto weigh = [&](const kv_f16& s, int t, auto AGAIN) {    // pair t begins, those before it go on; t = 0 .. 10
 #pragma unroll
-        for (int k = 3; k >= 0; k--) if (t - k >= 0 && t - k < 8) stage(s, t - k, k);
+        for (int k = 3; k >= 0; k--) if (t - k >= 0 && t - k < 8) stage(s, t - k, k, AGAIN);
     };
     // Scores of half tile b of tile c into n, while the weights of s are formed: spread over the KS steps of the product.  The first fragments of a product are
     // read from LDS in the last steps of the one before: vb_ is the half whose values come next.
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
             else vr[i + RING - KS] = value(vl, (i + RING - KS) >> 1, (i + RING - KS) & 1);
             if constexpr (WEIGH) {
 #pragma unroll
-                for (int t = 11 * i / KS; t < 11 * (i + 1) / KS; t++) weigh(s, t);
+                for (int t = 11 * i / KS; t < 11 * (i + 1) / KS; t++) weigh(s, t, no());
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= f;
 #pragma unroll
-            for (int t = 0; t < 11; t++) weigh(s, t);
+            for (int t = 0; t < 11; t++) weigh(s, t, yes());
         }
         l += hs;
     };
@@ -275,7 +280,6 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    using yes = std::integral_constant<bool, true>; using no = std::integral_constant<bool, false>;
     if (c0 < c1) {
         if (tid == 0) *Odd = 0;
 #pragma unroll

@@ -1,7 +1,6 @@
 """Operators over a caller's paged cache where numbers are hard: infinities, weights far below another, values near the end of the numbers, shares that are joined; the definition is
 tests/kv_reference.py."""
 import math
-import random
 
 import pytest
 import torch
@@ -224,3 +223,42 @@ def test_a_first_call_may_be_captured():
             torch.cuda.synchronize()
             agrees(got, q, cache, fmt, states, counts, 2.0 ** -16)
             assert torch.equal(got, batch.attend(0, q))
+
+
+# ---------------------------------------------------------------------------------------------------------------- scores
+@pytest.mark.parametrize("power", [20, 27, 30, 34, 40, 60])
+@pytest.mark.parametrize("fmt,dtype", [("bf16", "bf16"), ("f16", "f16"), ("mx8", "bf16"), ("mx8", "f16")])
+@pytest.mark.parametrize("dim,lens,counts", [(64, [90], [1]), (128, [200, 9000], [2, 1]), (128, [200], [40]), (64, [9000, 100], [33, 70])])
+def test_scores_of_any_size(fmt, dtype, dim, lens, counts, power):
+    """Scores of up to 2^power: one key draws all, as every other is far under it.  32 bits hold scores to 2^-24 of their size, no more; weights are those of the scores that 32 bits hold."""
+    cache = make_cache(2, dim, fmt, pages_for(lens, 16))
+    fill(cache, fmt, 1)
+    batch, states = batch_of(cache, lens, counts)
+    stored_poison(cache, fmt, states)
+    q = rows(sum(counts), 4, dim, DTYPES[dtype], 3)
+    got = batch.attend(0, q, scale=2.0 ** (power - 3)).double()
+    r = 0
+    for s, n in zip(states, counts):
+        k, v = stored_rows(cache, s, fmt)
+        see = visible(s.seq_len - n, n).cuda()
+        for h in range(4):
+            score = torch.where(see, q[r:r + n, h].double() @ k[:, h // 2].t().contiguous(), -math.inf)
+            top, at = score.topk(min(2, s.seq_len), -1)
+            # two keys within what sums of 32 bits leave of the products are not told apart; the others have to be
+            error = 2 * (dim + 16) * 2.0 ** -24 * (q[r:r + n, h].double().abs() @ k[:, h // 2].abs().t().contiguous()).amax(-1)
+            alone = (top[:, 0] - top[:, -1] - error) * 2.0 ** (power - 3) > 40.0 if top.shape[1] > 1 else torch.ones(n, dtype=torch.bool, device="cuda")
+            want = v[at[:, 0], h // 2]
+            assert int(alone.sum()) * 2 > n or n < 3, int(alone.sum())
+            assert bool(((got[r:r + n, h] - want).abs() <= torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -24)[alone].all()), (s.seq_len, n, h, got[r:r + n, h][alone][:, :4], want[alone][:, :4])
+            assert bool(got[r:r + n, h].isfinite().all())
+        r += n
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-41])
+def test_scales_of_next_to_nothing(scale):
+    lens, counts = [50, 300, 90], [1, 2, 40]
+    cache = make_cache(2, 64, "mx8", pages_for(lens, 16))
+    fill(cache, "mx8", 1)
+    batch, states = batch_of(cache, lens, counts)
+    q = rows(sum(counts), 4, 64, torch.bfloat16, 3)
+    agrees(batch.attend(0, q, scale=scale), q, cache, "mx8", states, counts, 2.0 ** -8, scale=scale)
