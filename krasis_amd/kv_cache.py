@@ -434,7 +434,7 @@ class KVBatch:
 
 def plan_of(cache: PagedKVCache, states: Sequence[SequenceKVState], counts: Sequence[int], stored: bool = False) -> torch.Tensor:
     """What the calls of a step share (kr_kv_plan in include/krasis_hip.h), on the host."""
-    ints = lambda x: torch.tensor(list(x), dtype=torch.int32)
+    ints = lambda x: torch.tensor(list(x), dtype=torch.int32, device="cpu")      # the library follows these: never on a program's default device
     lens = ints(s.seq_len + (0 if stored else c) for s, c in zip(states, counts))
     cnt, sizes, need = ints(counts), ints(len(s.pages) for s in states), ctypes.c_size_t()
     tables = array.array("i")                        # 32 sequences of 500 pages: 0.33 ms; through a tensor of a Python list 1.2
@@ -443,6 +443,6 @@ def plan_of(cache: PagedKVCache, states: Sequence[SequenceKVState], counts: Sequ
     lib = _lib.load_library()
     args = (cache.max_pages, cache.page_size, len(states), lens.data_ptr(), cnt.data_ptr(), tables.buffer_info()[0] if tables else lens.data_ptr(), sizes.data_ptr())
     _lib.check(lib.kr_kv_plan(*args, None, 0, ctypes.byref(need)))
-    plan = torch.empty(need.value, dtype=torch.int32)
+    plan = torch.empty(need.value, dtype=torch.int32, device="cpu")
     _lib.check(lib.kr_kv_plan(*args, plan.data_ptr(), need.value, ctypes.byref(need)))
     return plan

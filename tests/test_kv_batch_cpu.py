@@ -205,3 +205,13 @@ def test_a_callers_own_cache_object_is_unpaged_as_before():
     store = Store()
     (k, v), = unpage_into_store(store, s, [None, 0], 32)
     assert store.args[0] == 20 and torch.equal(torch.from_numpy(k.view("float16"))[:20], want) and not v.any()
+
+
+def test_plans_are_made_on_the_host_whatever_the_default_device():
+    from krasis_amd.kv_cache import plan_of
+    cache = make_cache(2, 64, "mx8", 16, device="cpu")
+    st = states(cache, [20, 5])
+    want = plan_of(cache, st, [3, 2])
+    with torch.device("meta"):                                      # a device whose addresses are 0: nothing is followed that is not there
+        got = plan_of(cache, st, [3, 2])
+    assert got.device.type == "cpu" and torch.equal(got, want)
