@@ -231,7 +231,8 @@ static int attend(const kr_kv_pages* p, const int* plan, const int* dev_plan, co
     if (int rc = check_attend(p, plan, heads, window, keep_first, parents != nullptr, a.p)) return rc;
     if (dtype != KR_KV_BF16 && dtype != KR_KV_F16) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: queries are bf16 or f16");
     if (bits_of(p->format) == 16 && p->format != dtype) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: queries of another 16-bit type than the pages");
-    if (!isfinite(scale)) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: scale %f", scale);
+    const float scale_log2 = scale * 1.44269504088896340736f;
+    if (!isfinite(scale_log2)) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: scale %g", scale);
     const Plan h(plan);
     if (!h.rows) return KR_OK;
     if (!dev_plan || !q || !out || misaligned(q) || misaligned(out)) return kr_fail(KR_ERR_VALUE, "kr_kv_attend: queries and output must be aligned to 16 bytes");
@@ -240,7 +241,7 @@ static int attend(const kr_kv_pages* p, const int* plan, const int* dev_plan, co
     a.q = (const uint16_t*)q; a.out = (uint16_t*)out; a.q_tok = q_token_stride; a.q_head = q_head_stride; a.parents = parents;
     a.heads = heads; a.kv_heads = kv_divisor((uint32_t)p->kv_heads); a.G = kv_divisor((uint32_t)(heads / p->kv_heads));
     a.window = window; a.first = clamp_first(h, window, keep_first);
-    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.scale_log2 = scale_log2;
     Part part[2];
     parts_of(h, p->kv_heads, heads, p->dim, fmt_of(p->format), dtype == KR_KV_F16, window, a.first, parents != nullptr, part);
     const size_t b0 = part_bytes(part[0], p->dim), b1 = part_bytes(part[1], p->dim);

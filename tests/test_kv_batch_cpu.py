@@ -215,3 +215,9 @@ def test_plans_are_made_on_the_host_whatever_the_default_device():
     with torch.device("meta"):                                      # a device whose addresses are 0: nothing is followed that is not there
         got = plan_of(cache, st, [3, 2])
     assert got.device.type == "cpu" and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale", [2.5e38, -3e38, float("inf")])
+def test_scales_that_end_the_numbers_are_refused(scale):
+    with pytest.raises(ValueError, match="scale"):
+        c_call(scale=scale)
