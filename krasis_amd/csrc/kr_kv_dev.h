@@ -19,11 +19,6 @@ __host__ __device__ __forceinline__ uint32_t kv_div(uint32_t x, KvDiv d, uint32_
 }
 __host__ __device__ __forceinline__ uint32_t kv_div(uint32_t x, KvDiv d) { uint32_t rest; return kv_div(x, d, rest); }
 __device__ __forceinline__ uint32_t kv_page(const KvPages& p, uint32_t j, uint32_t& off) { return kv_div(j, p.page, off); }
-__device__ __forceinline__ uint32_t kv_slot(const KvPages& p, const int* table, uint32_t j) {
-    uint32_t off;
-    const uint32_t n = kv_page(p, j, off);
-    return (uint32_t)table[n] * p.page.d + off;
-}
 
 // two neighbouring codes of a dword times the scale as a packed pair of bf16.  E4M3 and E2M1 have at most four significant bits and scales are powers of two of at least 2^-100:
 // every product is exact in bf16.

@@ -2,7 +2,7 @@
 // Writing quantises: a microscaled block of 32 channels gets the smallest power of two 2^s with max|x| <= M 2^s (M = 448 for E4M3, 6 for E2M1; s >= -100), its elements are
 // x / 2^s (exact) rounded to nearest even.  A block that holds a NaN or an infinity gets scale byte 255 and reads back as NaN.  All of it is bound by memory: a thread takes eight
 // channels (16 bytes of a row) at a time, four threads a block, whose maximum they find among themselves.  49863 tokens of two heads of 256 channels read back from eight bits to f16 (155 MB)
-// 24.4 us, 6.3 TB/s; three prompts of four heads of 128 stored at four bits 9.0 us and read back 7.8 (31 MB each).
+// 24.3 us, 6.3 TB/s; three prompts of four heads of 128 stored at four bits 8.9 us and read back 7.5 (31 MB each).
 #include "kr_kv_dev.h"
 
 constexpr int KV_UNITS = 4;

@@ -8,8 +8,11 @@
 // next half and the coming tiles' conversion go under the product with V; the first fragments of each product are read from LDS under the one before.
 // Weights are measured from a reference of the row (kr_kv_dev.h) that moves only when a half tile's sum of weights gets out of bounds.  No maxima are formed on the way, and O is hardly ever
 // rescaled.
-// Measured: two prompts of 8192 and 3001 tokens (64 / 4 heads of 128, eight bits) 1.03 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 46 % busy at the 1.9 GHz that its
-// power leaves; portions with heads of 256 channels over f16 pages 863 TFLOP/s, one wave a SIMD, 4.7 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
+// Weights are rounded to the products' type: bf16 to half a step of 2^-8, as far as the result is rounded itself, f16 2^-11; their sum is of the rounded ones, so that equal values come out as they
+// are.  A second bf16 piece would leave 2^-16 and half as many products again: two prompts of 8192 and 3001 tokens 1215 -> 1657 us, 64 drafts late in four documents 119 -> 157, a dozen of eight
+// chats 21.2 -> 21.9.  f16 queries over pages that become bf16 have two pieces of queries and weights.
+// Measured: those two prompts (64 / 4 heads of 128, eight bits) 1.03 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 47 % busy at the 1.9 GHz that its
+// power leaves; portions with heads of 256 channels over f16 pages 845 TFLOP/s, one wave a SIMD, 4.8 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
 // tile of 128 channels 1.3 us alone: short sequences are bound by that.
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
     }
     {
         l += __shfl_xor(l, 32);
-    if (rw + col >= rows) return;
+        if (rw + col >= rows) return;
         if (it.nsplit == 1) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint16_t* op = a.out + ((size_t)(it.row0 + tk) * a.heads + it.kvh * G + r - tk * G) * DIM + 4 * h;
