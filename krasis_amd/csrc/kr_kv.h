@@ -68,8 +68,9 @@ __host__ __device__ constexpr int kv_tile_waves(int dim, int fmt, bool half) {
 }
 // Waves of a workgroup in kr_kv_step_dev.h, one workgroup a CU.  one: every sequence has one new token: as many as the registers hold (half: f16 queries, two pieces over pages that become bf16).
 // Several new tokens take 8, and 4 from 192 channels on; by their registers they could take more (64 channels 127 to 142, 128 channels 158 to 193), which is not measured.
+// (Of 96 channels 16-bit pages take twelve: with sixteen two registers spill, 32 requests of up to 8192 tokens 57.4 us, 53.8 with twelve.)
 __host__ __device__ constexpr int kv_step_waves(int dim, int fmt, bool half, bool one) {
-    return !one ? (dim <= 128 ? 8 : 4) : dim == 64 || (dim == 96 && fmt == 0) || (dim == 128 && fmt == 2 && !half) ? 16 : dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8;
+    return !one ? (dim <= 128 ? 8 : 4) : dim == 64 || (dim == 128 && fmt == 2 && !half) ? 16 : dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8;
 }
 constexpr int KV_MAX_TREE = 64;                      // drafts of one sequence: their ancestors are a 64-bit word
 

@@ -136,23 +136,31 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& i
 }
 
 // ---- references of the softmax: weights are exp2(score - m), and m, -infinity until the row has seen a key, is no more than a measure that sums and weights share.  It stands while a lane's
-// sum of weights (of 8 keys or 16) lies in bounds and moves, with what was summed so far, when it does not.
-// f16 weights (HM) are subnormal numbers below 2^-14 and end at 2^16.  The reference is 2^-8 of the largest weight it was taken from, moves up when a sum passes 2^15, and down again when it
-// falls under 2^-6: a key may draw nearly all attention and be worth nothing, and the many far under it are the result.  So the largest weight of a tile's keys is 2^-10 at least, the others are
-// off by 2^-25 at most.  It stays within 2^60 of what was summed, where 32-bit sums of 16-bit numbers have their end far away.
+// sum of weights (of 8 keys or 16) lies in bounds and may move, with what was summed so far, when it does not.
 // bf16 weights have the range of 32 bits.  The reference is 2^8 times the largest weight it was taken from, and moves up when a sum passes 1: no weight is over 1, so that values up to the end of
 // the numbers have no larger sums than the definition gives them, and weights end at 2^-118 of the largest.
-template <bool HM> __device__ __forceinline__ bool kv_out_of_bounds(float sum, float most) { return sum > most || (HM && sum < 0.015625f); }
-// Weights are worked out as exp2(fma(product, scale, -m)), and once more where the reference moves: as exp2(score - m) of scores rounded to 32 bits, as m is.  Past 2^20 the rounding of m is no
+// f16 weights (HM) are subnormal numbers below 2^-14 and end at 2^16.  A reference goes up to 2^-10 of the largest weight when a lane's sum passes 2^15, so that no weight is off by more than
+// 2^-35 of the row's largest.  A key may draw nearly all attention and be worth nothing, though, and the many far under it are the result: when a lane's sum falls under 2^-10 (16 equal weights are
+// 2^-14 each) the reference comes down, as far as the tile's largest key allows, and its weights are off by 2^-11 of their sum again.  It stays within 2^60 of what was summed, where 32-bit sums of
+// 16-bit numbers have their end far away, and comes down four times at most in a wave's share of the keys: scores that vary by more than the 2^25 between the bounds would move it to and fro
+// (portions of f16 pages, queries 1, 2, 3, 5 and 10 times as large: 1.72, 1.64, 1.83, 1.73, 1.71 ms; down without end 1.75, 2.10, 2.32, 2.33, 2.33; never down 1.74, 1.66, 1.64, 1.61, 1.62).
+// Weights are worked out as exp2(fma(product, scale, -m)), and once more where a reference moves: as exp2(score - m) of scores rounded to 32 bits, as m is.  Past 2^20 the rounding of m is no
 // longer small, and would be all that a weight from the fma is made of past 2^27: there all weights are worked out twice.
-// most: -1, which every sum passes, until the row has seen a key, and for references past 2^20
+struct KvBounds { float most, least; };      // of a lane's sum.  most: -1, which every sum passes, until the row has seen a key, and for references past 2^20; least: 0 where it comes down no more
+constexpr float KV_LEAST = 0x1p-10f;
+template <bool HM> __device__ __forceinline__ bool kv_out_of_bounds(float sum, const KvBounds& b) { return sum > b.most || (HM && sum < b.least); }
 template <bool HM> __device__ __forceinline__ float kv_most(float m) { return fabsf(m) > 1048576.0f ? -1.0f : HM ? 32768.0f : 1.0f; }
-// the reference after keys whose largest score is t; sum: all of the row's weights so far
-template <bool HM> __device__ __forceinline__ float kv_reference(float m, float t, float sum) {
+// the reference after keys whose largest score is t, in one lane no more than low; sum: all of the row's weights so far
+template <bool HM> __device__ __forceinline__ float kv_reference(float m, float t, float low, float sum, KvBounds& b) {
     if constexpr (!HM) return fmaxf(m, t + 8.0f);
     else {
-        const float low = t - 8.0f;                          // past 2^27 the numbers lie 16 apart
-        return t != -INFINITY && (t - m > 8.0f || m - t > 6.0f) ? fmaxf(t - low > 8.0f ? t : low, m + __builtin_amdgcn_logf(sum) - 60.0f) : m;
+        if (t == -INFINITY) return m;
+        const float ten = t - 10.0f, under = t - ten > 10.0f ? t : ten;      // past 2^27 the numbers lie 16 apart
+        if (t - m > 10.0f) return under;
+        const float end = m + __builtin_amdgcn_logf(sum) - 60.0f, to = fmaxf(fmaxf(low + 8.0f, under), end);
+        if (!(m - low > 10.0f && to < m - 2.0f && b.least > 0.0f)) return m;
+        b.least = to == end ? 0.0f : b.least - KV_LEAST / 4;
+        return to;
     }
 }
 

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
     };
 
     const float scale = fmaxf(fabsf(a.scale_log2), 1.1754944e-38f);      // its sign goes into the queries: scores that are not seen are -infinity before it, too
-    float m = -INFINITY, l = 0.0f, base = 0.0f, most = -1.0f;
+    float m = -INFINITY, l = 0.0f, base = 0.0f; KvBounds bounds = {-1.0f, KV_LEAST};
     kv_f4 acc[DIM / 16];
 #pragma unroll
     for (int j = 0; j < DIM / 16; j++) acc[j] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -198,20 +198,25 @@ __global__ void __launch_bounds__(64 * kv_step_waves(DIM, FMT, HQ, ONE), kv_step
             }
         };
         weigh(std::integral_constant<bool, false>());
-        if (__any(kv_out_of_bounds<HM>(hs, most))) {
+        if (__any(kv_out_of_bounds<HM>(hs, bounds))) {
             float t = st[0][0];
 #pragma unroll
             for (int i = 1; i < 8; i++) t = fmaxf(t, st[i >> 2][i & 3]);
+            float low = t == -INFINITY ? INFINITY : t, sum = l;
             t = fmaxf(t, __shfl_xor(t, 16)); t = fmaxf(t, __shfl_xor(t, 32));
-            float sum = l;
-            if constexpr (HM) { sum += __shfl_xor(sum, 16); sum += __shfl_xor(sum, 32); }
-            const float mn = kv_reference<HM>(m, t * scale, sum);
-            base = mn == -INFINITY ? 0.0f : mn;
-            const float f = __builtin_amdgcn_exp2f(m - base);
-            m = mn; l *= f; most = kv_most<HM>(mn);
+            if constexpr (HM) {
+                low = fminf(low, __shfl_xor(low, 16)); low = fminf(low, __shfl_xor(low, 32));
+                sum += __shfl_xor(sum, 16); sum += __shfl_xor(sum, 32);
+            }
+            const float mn = kv_reference<HM>(m, t * scale, low * scale, sum, bounds);
+            if (__any(mn != m || bounds.most < 0.0f)) {
+                base = mn == -INFINITY ? 0.0f : mn;
+                const float f = __builtin_amdgcn_exp2f(m - base);
+                m = mn; l *= f; bounds.most = kv_most<HM>(mn);
 #pragma unroll
-            for (int j = 0; j < DIM / 16; j++) acc[j] *= f;
-            weigh(std::integral_constant<bool, true>());
+                for (int j = 0; j < DIM / 16; j++) acc[j] *= f;
+                weigh(std::integral_constant<bool, true>());
+            }
         }
         l += hs;
         constexpr uint32_t EXP = HM ? 0x7C00u : 0x7F80u, UNIT = HM ? 0x3C00u : 0x3F80u;

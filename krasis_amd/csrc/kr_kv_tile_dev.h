@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
         }
         if (odd) *Odd = 1;
     };
-    float m = -INFINITY, l = 0.0f, base = 0.0f, hs = 0.0f, most = -1.0f;
+    float m = -INFINITY, l = 0.0f, base = 0.0f, hs = 0.0f; KvBounds bounds = {-1.0f, KV_LEAST};
     kv_f16 o[DB], sa, sb;
     u32x4 pf[NP][2];
 #pragma unroll
@@ -241,26 +241,32 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : kv_tile_waves(DIM, FMT, H
 #pragma unroll
         for (int i = 0; i < 16; i++) if (!(ok >> ((i & 3) + 8 * (i >> 2)) & 1)) s[i] = -INFINITY;
     };
+    auto halves = [&](float x) {                              // the wave's lower half and its upper one, a register each (through LDS the exchange waits for a round trip)
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return make_float2(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    };
     // The weights stand when no sum of a half tile is out of bounds; else, and until a row has seen its first key, the references move, and what was summed so far with them.  NaN scores
     // move nothing and are in the sums.
     auto settle = [&](const kv_f16& s) {
-        if (__any(kv_out_of_bounds<HM>(hs, most))) {
+        if (__any(kv_out_of_bounds<HM>(hs, bounds))) {
             float t = s[0];
 #pragma unroll
             for (int i = 1; i < 16; i++) t = fmaxf(t, s[i]);
-            t = fmaxf(t, __shfl_xor(t, 32)) * scale;
-            float sum = l;
-            if constexpr (HM) sum += __shfl_xor(sum, 32);
-            const float mn = kv_reference<HM>(m, t, sum);
-            base = mn == -INFINITY ? 0.0f : mn;
-            const float f = __builtin_amdgcn_exp2f(m - base);
-            m = mn; l *= f; most = kv_most<HM>(mn);
+            const auto ts = halves(t), ls = halves(l);         // of the row's two lanes
+            t = fmaxf(ts.x, ts.y);
+            const float low = ts.x == -INFINITY ? ts.y : ts.y == -INFINITY ? ts.x : fminf(ts.x, ts.y), sum = ls.x + ls.y;
+            const float mn = kv_reference<HM>(m, t * scale, low * scale, sum, bounds);
+            if (__any(mn != m || bounds.most < 0.0f)) {
+                base = mn == -INFINITY ? 0.0f : mn;
+                const float f = __builtin_amdgcn_exp2f(m - base);
+                m = mn; l *= f; bounds.most = kv_most<HM>(mn);
 #pragma unroll
-            for (int d = 0; d < DB; d++)
+                for (int d = 0; d < DB; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] *= f;
+                    for (int i = 0; i < 16; i++) o[d][i] *= f;
 #pragma unroll
-            for (int t = 0; t < 11; t++) weigh(s, t, yes());
+                for (int t = 0; t < 11; t++) weigh(s, t, yes());
+            }
         }
         l += hs;
     };

@@ -24,6 +24,8 @@ def agrees(got, q, cache, fmt, states, counts, weight, scale=None, window=0, fir
         if not k.isfinite().all():                                  # how large scores are, of keys that are numbers
             size = attend(q[r:r + n].double(), k.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), v.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0), see, scale)[2]
         tol = tolerance(out, mean, size, dim, s.seq_len, q.dtype, weight)
+        # denominators may be sums of the rounded weights p (1 + d), |d| <= weight: sum p (1 + d) v / sum p (1 + d) is off by sum p d (v - out) / sum p (1 + d), at most weight (mean + |out|)
+        tol = tol + weight * out.abs()
         # a weight under 2^-118 of the row's largest is 0 (kv_reference leaves 2^-8 of the range of 32 bits): off by less than that of its |v|, and a product under 2^-118 likewise
         tol = tol + s.seq_len * 2.0 ** -118 * (v[v.isfinite()].abs().max() + 1)
         if fmt == "f16":                                            # subnormal weights are off by 2^-25; the row's largest weighs 2^8 or more
