@@ -59,15 +59,15 @@ constexpr int KV_MAX_SHARES = 1024;                  // of a row tile
 
 constexpr int KV_STEP_BM = 16, KV_STEP_KT = 32;      // rows (new tokens x heads of a group) and keys of a tile in kr_kv_step_dev.h
 constexpr int KV_TILE_KT = 64;                       // keys of a tile in kr_kv_tile_dev.h; 32 rows a wave
-// Waves that a SIMD holds of the latter, by measurement.  Heads of 64 channels take three under bf16 queries over eight and four bits, though 10 and 3 registers do not fit into 168: two prompts
+// Waves that a SIMD holds of the latter, by measurement.  Heads of 64 channels take three under bf16 queries over eight and four bits, though 4 and 8 registers do not fit into 168: two prompts
 // of 8192 and 3001 tokens 405 -> 382 us.  Others would spill more: 16-bit pages 390 us with two, 498 with three, f16 queries over eight bits 595 and 690.
-// Of 128 channels (four waves a workgroup) f16 queries over eight bits take one: 64 sequences' drafts 96 us with one, 122 with two; over four bits 96 and 82, 16-bit pages, of which 8 registers
-// spill, 82 and 79.  Eight waves a workgroup are two a SIMD: 6 registers of f16 queries over four bits spill.
+// Of 128 channels (four waves a workgroup) f16 queries over eight bits take one: 64 sequences' drafts 96 us with one, 122 with two; over four bits 96 and 82, 16-bit pages, of which 7 registers
+// spill, 82 and 79.  Eight waves a workgroup are two a SIMD: 5 registers of f16 queries over four bits spill.
 __host__ __device__ constexpr int kv_tile_waves(int dim, int fmt, bool half) {
     return dim == 64 && fmt != 0 && !half ? 3 : dim < 128 || (dim == 128 && !(fmt == 1 && half)) ? 2 : 1;
 }
 // Waves of a workgroup in kr_kv_step_dev.h, one workgroup a CU.  one: every sequence has one new token: as many as the registers hold (half: f16 queries, two pieces over pages that become bf16).
-// Several new tokens take 8, and 4 from 192 channels on; by their registers they could take more (64 channels 127 to 142, 128 channels 158 to 193), which is not measured.
+// Several new tokens take 8, and 4 from 192 channels on; by their registers they could take more (64 channels 128 to 142, 128 channels 158 to 193), which is not measured.
 // (Of 96 channels 16-bit pages take twelve: with sixteen two registers spill, 32 requests of up to 8192 tokens 57.4 us, 53.8 with twelve.)
 __host__ __device__ constexpr int kv_step_waves(int dim, int fmt, bool half, bool one) {
     return !one ? (dim <= 128 ? 8 : 4) : dim == 64 || (dim == 128 && fmt == 2 && !half) ? 16 : dim <= 128 ? 12 : dim == 256 && fmt == 0 ? 4 : 8;

@@ -138,7 +138,8 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, const KvItem& i
 // ---- references of the softmax: weights are exp2(score - m), and m, -infinity until the row has seen a key, is no more than a measure that sums and weights share.  It stands while a lane's
 // sum of weights (of 8 keys or 16) lies in bounds and may move, with what was summed so far, when it does not.
 // bf16 weights have the range of 32 bits.  The reference is 2^8 times the largest weight it was taken from, and moves up when a sum passes 1: no weight is over 1, so that values up to the end of
-// the numbers have no larger sums than the definition gives them, and weights end at 2^-118 of the largest.
+// the numbers have no larger sums than the definition gives them, and weights end at 2^-118 of the largest
+// (two prompts over eight bits, queries 1, 2, 3, 5 and 10 times as large: 1.29, 1.24, 1.30, 1.35, 1.40 ms; weights of up to 2^30, which moved it less, 1.34, 1.26, 1.27, 1.28, 1.32).
 // f16 weights (HM) are subnormal numbers below 2^-14 and end at 2^16.  A reference goes up to 2^-10 of the largest weight when a lane's sum passes 2^15, so that no weight is off by more than
 // 2^-35 of the row's largest.  A key may draw nearly all attention and be worth nothing, though, and the many far under it are the result: when a lane's sum falls under 2^-10 (16 equal weights are
 // 2^-14 each) the reference comes down, as far as the tile's largest key allows, and its weights are off by 2^-11 of their sum again.  It stays within 2^60 of what was summed, where 32-bit sums of

@@ -7,7 +7,7 @@
 // A workgroup takes one sequence, one key / value head and a share of its key tiles; its waves, as many as a CU has registers for, take tiles of 32 keys in turn, each with a reference and a sum per row, and
 // meet in LDS.  Over pages that become bf16 weights are two bf16 pieces (off by 2^-16), and so are f16 queries; over f16 pages weights are f16 (2^-11, as the result is rounded itself).
 // (One piece is no faster where memory bounds the launch: 32 requests of up to 8192 tokens 43.4 us a call with either, two of 131071 and 100003 40.5 and 40.7.)
-// Measured: 32 requests of up to 8192 tokens at eight bits (142 MB) 31.1 us, 4.6 TB/s, two of 131071 and 100003 at four bits (126 MB) 31.5 us, 4.0 TB/s; 97 tokens of a chat 7 us, which is one
+// Measured: 32 requests of up to 8192 tokens at eight bits (142 MB) 31.3 us, 4.5 TB/s, two of 131071 and 100003 at four bits (126 MB) 32.1 us, 3.9 TB/s; 97 tokens of a chat 7 us, which is one
 // round trip after the other (arguments, plan, page table, keys).
 #pragma once
 #include "kr_kv_dev.h"

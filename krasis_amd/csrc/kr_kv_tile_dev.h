@@ -11,8 +11,8 @@
 // Weights are rounded to the products' type: bf16 to half a step of 2^-8, as far as the result is rounded itself, f16 2^-11; their sum is of the rounded ones, so that equal values come out as they
 // are.  A second bf16 piece would leave 2^-16 and half as many products again: two prompts of 8192 and 3001 tokens 1215 -> 1657 us, 64 drafts late in four documents 119 -> 157, a dozen of eight
 // chats 21.2 -> 21.9.  f16 queries over pages that become bf16 have two pieces of queries and weights.
-// Measured: those two prompts (64 / 4 heads of 128, eight bits) 1.03 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 47 % busy at the 1.9 GHz that its
-// power leaves; portions with heads of 256 channels over f16 pages 845 TFLOP/s, one wave a SIMD, 4.8 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
+// Measured: those two prompts (64 / 4 heads of 128, eight bits) 1.02 PFLOP/s where a library product of 8192^3 reaches 1.21, the matrix pipe 47 % busy at the 1.9 GHz that its
+// power leaves; portions with heads of 256 channels over f16 pages 850 TFLOP/s, one wave a SIMD, 4.8 vector instructions a matrix instruction.  A workgroup's start takes 3 us and up, a
 // tile of 128 channels 1.3 us alone: short sequences are bound by that.
 #include "kr_kv_dev.h"
 #include "kr_lds_optin.h"
